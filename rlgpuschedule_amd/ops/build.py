@@ -16,6 +16,12 @@ OUT = PKG / "ops"
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = os.environ.get("RLS_OFFLOAD_ARCH", "gfx950")
 
+# Packed FP32 instructions stay off: hipcc -O3 forms them from ordinary float
+# code, and some of their forms have given wrong results on this part.
+# (hipcc's host pass warns that it does not know the feature; harmless.)
+FLAGS = ["-O3", "-std=c++17", "-fPIC", "-shared",
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+
 # name -> sources
 _LIBS = {
     "librlsched_env.so": ["env_step.hip"],
@@ -27,12 +33,12 @@ _LIBS = {
 
 
 def source_hash(name: str) -> str:
-    """sha256-prefix over this lib's sources + all shared headers.
-    Embedded at compile time (-DRLS_SOURCE_HASH) and checked at load:
-    a committed .so whose sources changed can never silently test old
-    kernels (VERDICT r1 weak #6)."""
+    """sha256-prefix over this lib's sources + all shared headers + the
+    compile flags. Embedded at compile time (-DRLS_SOURCE_HASH) and checked
+    at load: a .so whose sources changed can never silently test old
+    kernels."""
     import hashlib
-    h = hashlib.sha256()
+    h = hashlib.sha256(" ".join(FLAGS).encode())
     srcs = [CSRC / s for s in _LIBS[name]] + sorted(CSRC.glob("*.h"))
     for p in sorted(srcs):
         h.update(p.name.encode())
@@ -59,24 +65,27 @@ def _needs_build(so: Path, srcs: list[Path], name: str) -> bool:
     return embedded_hash(so) != source_hash(name)
 
 
-def build_lib(name: str, verbose: bool = False) -> Path:
+def build_lib(name: str, verbose: bool = False, force: bool = False) -> Path:
     srcs = [CSRC / s for s in _LIBS[name]]
     missing = [s for s in srcs if not s.exists()]
     if missing:
         raise FileNotFoundError(f"missing sources for {name}: {missing}")
     so = OUT / name
-    if not _needs_build(so, srcs, name):
+    if not force and not _needs_build(so, srcs, name):
         return so
     h = source_hash(name)
+    tmp = so.with_suffix(f".{os.getpid()}.tmp")   # replaced whole, when done
     cmd = [
-        HIPCC, f"--offload-arch={ARCH}", "-O3", "-std=c++17",
-        "-fPIC", "-shared", f'-DRLS_SOURCE_HASH="{h}"', "-o", str(so),
+        HIPCC, f"--offload-arch={ARCH}", *FLAGS,
+        f'-DRLS_SOURCE_HASH="{h}"', "-o", str(tmp),
     ] + [str(s) for s in srcs]
     if verbose:
         print("+", " ".join(cmd))
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
+        tmp.unlink(missing_ok=True)
         raise RuntimeError(f"hipcc failed for {name}:\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, so)
     got = embedded_hash(so)
     if got != h:
         raise RuntimeError(f"{name}: embedded hash {got!r} != expected {h!r} "
@@ -104,12 +113,14 @@ def verify_loaded(lib, name: str) -> None:
             f"{want}; the mapped binary does not match csrc/ — rebuild")
 
 
-def build_all(verbose: bool = False) -> list[Path]:
-    out = []
-    for name, srcs in _LIBS.items():
-        if all((CSRC / s).exists() for s in srcs):
-            out.append(build_lib(name, verbose))
-    return out
+def build_all(verbose: bool = False, force: bool = False) -> list[Path]:
+    """Build every library (force: also those whose binary is current),
+    a few compilers at a time."""
+    from concurrent.futures import ThreadPoolExecutor
+    names = [name for name, srcs in _LIBS.items()
+             if all((CSRC / s).exists() for s in srcs)]
+    with ThreadPoolExecutor(max_workers=4) as pool:
+        return list(pool.map(lambda n: build_lib(n, verbose, force), names))
 
 
 if __name__ == "__main__":
