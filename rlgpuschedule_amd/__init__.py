@@ -8,7 +8,8 @@ and IMPALA-style async actor/learner, with data parallelism over RCCL/xGMI.
 Public API (lazy imports; heavy deps load on first use):
     EnvSpec, cluster16/64/256/1024, ClusterSchedEnv, CpuVectorEnv,
     HipVectorEnv, MLPPolicy, GRUPolicy, TrainConfig, CONFIGS, train,
-    JobTrace, philly_like, poisson
+    JobTrace, philly_like, poisson,
+    layer_norm, gated_scan, gated_scan_step, action_logprobs
 """
 __version__ = "0.1.0"
 
@@ -29,6 +30,10 @@ _EXPORTS = {
     "JobTrace": "rlgpuschedule_amd.traces.synthetic",
     "philly_like": "rlgpuschedule_amd.traces.synthetic",
     "poisson": "rlgpuschedule_amd.traces.synthetic",
+    "layer_norm": "rlgpuschedule_amd.ops.norm",
+    "gated_scan": "rlgpuschedule_amd.ops.scan",
+    "gated_scan_step": "rlgpuschedule_amd.ops.scan",
+    "action_logprobs": "rlgpuschedule_amd.ops.logprob",
 }
 
 

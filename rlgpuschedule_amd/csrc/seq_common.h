@@ -1,0 +1,78 @@
+// Shared pieces of the sequence operators (layer_norm.hip, gated_scan.hip,
+// logprob.hip): element types, wide loads and stores, wave reductions, and
+// launches that stay on the caller's device and stream.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+namespace seq {
+
+constexpr int kWave = 64;
+
+// element type codes, as ops/_seq.py passes them
+enum Type { F32 = 0, BF16 = 1, F16 = 2 };
+
+typedef __bf16 bf16;
+typedef _Float16 f16;
+
+// N elements as one load or store of N * sizeof(T) bytes (at most 16)
+template <typename T, int N>
+struct alignas(sizeof(T) * N) Vec {
+  T v[N];
+};
+
+template <typename T, int N>
+__device__ __forceinline__ void load(const T* p, float (&f)[N]) {
+  Vec<T, N> r = *reinterpret_cast<const Vec<T, N>*>(p);
+#pragma unroll
+  for (int i = 0; i < N; ++i) f[i] = (float)r.v[i];
+}
+
+// One rounding to nearest even, of a value held in 32 bits.
+template <typename T, int N>
+__device__ __forceinline__ void store(T* p, const float (&f)[N]) {
+  Vec<T, N> r;
+#pragma unroll
+  for (int i = 0; i < N; ++i) r.v[i] = (T)f[i];
+  *reinterpret_cast<Vec<T, N>*>(p) = r;
+}
+
+template <int W = kWave>
+__device__ __forceinline__ float group_sum(float v) {
+#pragma unroll
+  for (int o = W / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, kWave);
+  return v;
+}
+
+// Runs the scope on one device and goes back to the caller's.
+struct OnDevice {
+  int before = -1;
+  hipError_t err;
+  explicit OnDevice(int device) {
+    err = hipGetDevice(&before);
+    if (err == hipSuccess && before != device) {
+      err = hipSetDevice(device);
+    } else {
+      before = -1;
+    }
+  }
+  ~OnDevice() {
+    if (before >= 0) (void)hipSetDevice(before);
+  }
+};
+
+// The launch's own status: an error left by other code stays where it is.
+template <typename... P, typename... A>
+inline hipError_t launch(void (*kernel)(P...), dim3 grid, dim3 block,
+                         size_t lds, hipStream_t stream, A... args) {
+  void* list[] = {(void*)&args...};
+  static_assert(sizeof...(P) == sizeof...(A), "one value for each parameter");
+  return hipLaunchKernel((const void*)kernel, grid, block, list, lds, stream);
+}
+
+inline bool aligned(const void* p, int64_t bytes) {
+  return ((uintptr_t)p & (uintptr_t)(bytes - 1)) == 0;
+}
+
+}  // namespace seq

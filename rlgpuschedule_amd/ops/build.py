@@ -29,6 +29,9 @@ _LIBS = {
     "librlsched_train.so": ["train_kernels.hip"],
     "librlsched_gru.so": ["gru_train.hip"],
     "librlsched_mega.so": ["rollout_mega.hip"],
+    "librlsched_norm.so": ["layer_norm.hip"],
+    "librlsched_scan.so": ["gated_scan.hip"],
+    "librlsched_logp.so": ["logprob.hip"],
 }
 
 

@@ -1,0 +1,940 @@
+"""Sequence operators: layer norm, gated scan, action log probabilities.
+
+Each is held to its definition in 64 bits, written here apart from the
+package's references, with bounds counted from roundings: u = 2^-24 for each
+32-bit operation, half a step of the output's type for its one rounding, and
+a sum of L sequential additions off by at most L u times the sum of its
+terms' magnitudes."""
+import math
+
+import pytest
+import torch
+
+from rlgpuschedule_amd import (action_logprobs, gated_scan, gated_scan_step,
+                               layer_norm)
+from rlgpuschedule_amd.ops.logprob import (action_logprobs_bwd,
+                                           action_logprobs_fwd)
+from rlgpuschedule_amd.ops.norm import layer_norm_bwd, layer_norm_fwd
+from rlgpuschedule_amd.ops.scan import gated_scan_bwd, gated_scan_fwd
+
+U = 2.0 ** -24
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+TYPES = [F32, BF16, F16]
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def randn(g, *shape, dtype=F32, device="cpu", scale=1.0, shift=0.0):
+    return (torch.randn(*shape, generator=g) * scale + shift).to(
+        dtype).to(device)
+
+
+def half_step(t, dtype):
+    """Half a step of dtype at t's values, down to its subnormals."""
+    f = torch.finfo(dtype)
+    return t.abs() * (f.eps / 2) + f.smallest_normal * f.eps + 1e-36
+
+
+def close(got, want, tol, what):
+    got = got.detach().double().cpu()
+    assert got.shape == want.shape, what
+    same = (got == want) | (got.isnan() & want.isnan())
+    off = ((got - want).abs() - tol).masked_fill(same, -1.0)
+    assert not (off > 0).any() and not (off.isnan()).any(), (
+        f"{what}: {int((~(off <= 0)).sum())} of {off.numel()} off, worst "
+        f"{(got - want).abs()[~same].max():.3g}")
+
+
+# ---------------------------------------------------------------- layer norm
+def norm_64(x, w, b, eps, dy=None):
+    """Values and bounds of y (and dx, dw, db) in 64 bits, rows [n, d]."""
+    dt, wt = x.dtype, (w if w is not None else x).dtype
+    x = x.detach().double().cpu().reshape(-1, x.shape[-1])
+    n, d = x.shape
+    w = torch.ones(d).double() if w is None else w.detach().double().cpu()
+    b = torch.zeros(d).double() if b is None else b.detach().double().cpu()
+    mean = x.sum(1, keepdim=True) / d
+    r = 1 / (((x - mean) ** 2).sum(1, keepdim=True) / d + eps).sqrt()
+    nx = (x - mean) * r
+    y = nx * w + b
+    # a row's sums: at most d / 32 additions in a lane and 16 between lanes
+    L = (16 + d / 32) * U
+    # |x - mean| is off by the mean's error and one rounding; r by half of the
+    # variance's, whose terms' errors are 2 |x - mean| dmean
+    size = r * (x.abs() + x.abs().sum(1, keepdim=True) / d)
+    dn = (L + 4 * U) * size + (L + 6 * U) * nx.abs() * (
+        1 + size.pow(2).sum(1, keepdim=True) / d)
+    out = {"y": (y, half_step(y, dt) + dn * w.abs()
+                 + 2 * U * (nx.abs() * w.abs() + b.abs()))}
+    if dy is not None:
+        dy = dy.detach().double().cpu().reshape(n, d)
+        g = dy * w
+        s1, s2 = g.sum(1, keepdim=True) / d, (g * nx).sum(1, keepdim=True) / d
+        dx = r * (g - s1 - nx * s2)
+        ag = g.abs().sum(1, keepdim=True) / d
+        agn = (g * nx).abs().sum(1, keepdim=True) / d
+        ds2 = (L + 4 * U) * agn + (g.abs() * dn).sum(1, keepdim=True) / d
+        tol = r * ((L + 6 * U) * (g.abs() + ag + nx.abs() * agn)
+                   + dn * s2.abs() + (nx.abs() + dn) * ds2)
+        # r's own relative error multiplies the whole, before cancellation
+        tol = tol + (L + 6 * U) * r * (g.abs() + s1.abs() + (nx * s2).abs()) \
+            * (1 + size.pow(2).sum(1, keepdim=True) / d)
+        out["dx"] = (dx, half_step(dx, dt) + tol)
+        R = (64 + n) * U
+        dw, db = (dy * nx).sum(0), dy.sum(0)
+        out["dw"] = (dw, half_step(dw, wt) + (R * dy.abs() * nx.abs()).sum(0)
+                     + (dy.abs() * dn).sum(0))
+        out["db"] = (db, half_step(db, wt) + R * dy.abs().sum(0))
+    return out
+
+
+NORM_SIZES = [(1, 1), (3, 2), (5, 17), (64, 64), (7, 84), (33, 100),
+              (130, 256), (9, 263), (4, 1000), (17, 1021), (3, 2048),
+              (2, 4096), (3, 5001), (2, 8192), (2, 16392), (1, 40001),
+              (700, 24), (2100, 256)]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,dim", NORM_SIZES)
+def test_norm(device, dtype, rows, dim):
+    g = gen(rows * 31 + dim)
+    for wt in {dtype, F32}:
+        x = randn(g, rows, dim, dtype=dtype, device=device, shift=0.5)
+        w = randn(g, dim, dtype=wt, device=device, scale=0.3, shift=1.0)
+        b = randn(g, dim, dtype=wt, device=device)
+        dy = randn(g, rows, dim, dtype=dtype, device=device)
+        for t in (x, w, b):
+            t.requires_grad_(True)
+        y = layer_norm(x, w, b)
+        assert y.dtype == dtype
+        dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+        assert (dx.dtype, dw.dtype, db.dtype) == (dtype, wt, wt)
+        want = norm_64(x, w, b, 1e-5, dy)
+        for name, got in (("y", y), ("dx", dx), ("dw", dw), ("db", db)):
+            close(got, *want[name], f"{name} {rows}x{dim} {dtype} {wt}")
+        with torch.no_grad():
+            assert torch.equal(layer_norm(x, w, b), y)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("which", ["none", "weight", "bias"])
+def test_norm_without_weight_or_bias(device, which):
+    g = gen(3)
+    x = randn(g, 4, 5, 72, device=device).requires_grad_(True)
+    w = randn(g, 72, device=device).requires_grad_(True)
+    dy = randn(g, 4, 5, 72, device=device)
+    kw = {} if which == "none" else {which: w}
+    y = layer_norm(x, eps=1e-3, **kw)
+    want = norm_64(x, kw.get("weight"), kw.get("bias"), 1e-3, dy)
+    grads = torch.autograd.grad(y, (x, w) if kw else (x,), dy)
+    close(y.reshape(20, 72), *want["y"], "y")
+    close(grads[0].reshape(20, 72), *want["dx"], "dx")
+    if kw:
+        close(grads[1], *want["dw" if which == "weight" else "db"], which)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_norm_needs_only_what_is_asked(device):
+    g = gen(4)
+    x, w, b = randn(g, 6, 40, device=device), randn(
+        g, 40, device=device), randn(g, 40, device=device)
+    dy = randn(g, 6, 40, device=device)
+    want = norm_64(x, w, b, 1e-5, dy)
+    for i, name in enumerate(("dx", "dw", "db")):
+        leaves = [x.clone(), w.clone(), b.clone()]
+        leaves[i].requires_grad_(True)
+        got, = torch.autograd.grad(layer_norm(*leaves), leaves[i], dy)
+        close(got, *want[name], name)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+def test_norm_layouts(device, dtype):
+    """Strided, overlapping and misaligned rows, of inputs and gradients."""
+    g = gen(5)
+    wide = randn(g, 9, 2, 300, dtype=dtype, device=device)
+    flat = randn(g, 9 * 2 * 128 + 3, dtype=dtype, device=device)
+    w, b = (randn(g, 128, device=device) for _ in range(2))
+    views = [wide[:, :, :128], wide[:, :, 1:129], wide[:, 1, 5:133],
+             wide.transpose(0, 1)[:, :, 8:136], flat[3:].view(9, 2, 128),
+             wide[:, :1, :128].expand(9, 4, 128),
+             randn(g, 128, 9, dtype=dtype, device=device).t(),
+             wide[0, 0, :128]]
+    for k, v in enumerate(views):
+        dy = randn(g, *v.shape[:-1], 1, dtype=dtype,
+                   device=device).expand(v.shape)
+        x = v.detach().requires_grad_(True)
+        y = layer_norm(x, w, b)
+        dx, = torch.autograd.grad(y, x, dy)
+        want = norm_64(v, w, b, 1e-5, dy)
+        close(y.reshape(-1, 128), *want["y"], f"y of view {k}")
+        close(dx.reshape(-1, 128), *want["dx"], f"dx of view {k}")
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_norm_edges(device):
+    x = torch.zeros(0, 12, device=device, requires_grad=True)
+    w = torch.ones(12, device=device, requires_grad=True)
+    y = layer_norm(x, w, None)
+    assert y.shape == (0, 12)
+    dx, dw = torch.autograd.grad(y, (x, w), torch.zeros_like(y))
+    assert dx.shape == (0, 12) and torch.equal(dw, torch.zeros_like(dw))
+    # equal values have no variance: y is the bias
+    b = torch.arange(12.0, device=device)
+    assert torch.equal(layer_norm(torch.full((3, 12), 7.0, device=device), w,
+                                  b), b.expand(3, 12))
+    # one row's infinities and NaN stay in that row
+    x = torch.randn(3, 12).to(device)
+    bad = x.clone()
+    bad[1, 4] = math.inf
+    bad[2, 5] = math.nan
+    y = layer_norm(bad)
+    assert torch.equal(y[0], layer_norm(x)[0]) and y[1:].isnan().all()
+    # large means beside a small spread: the spread survives
+    big = torch.randn(2, 4096).to(device) + 3000.0
+    close(layer_norm(big), *norm_64(big, None, None, 1e-5)["y"], "shifted")
+
+
+def test_norm_refusals():
+    x = torch.zeros(4, 8)
+    cases = [
+        (ValueError, lambda: layer_norm_fwd(torch.zeros(()))),
+        (ValueError, lambda: layer_norm_fwd(torch.zeros(4, 0))),
+        (TypeError, lambda: layer_norm_fwd(torch.zeros(4, 8).long())),
+        (TypeError, lambda: layer_norm_fwd(x.double())),
+        (ValueError, lambda: layer_norm_fwd(x, torch.zeros(7))),
+        (ValueError, lambda: layer_norm_fwd(x, torch.zeros(1, 8))),
+        (TypeError, lambda: layer_norm_fwd(x, torch.zeros(8).half())),
+        (TypeError, lambda: layer_norm_fwd(
+            x.half(), torch.zeros(8).half(), torch.zeros(8))),
+        (ValueError, lambda: layer_norm_fwd(x, torch.zeros(8, device="meta"))),
+        (ValueError, lambda: layer_norm_bwd(
+            torch.zeros(4, 7), x, None, torch.zeros(4), torch.zeros(4))),
+        (ValueError, lambda: layer_norm_bwd(
+            x.half(), x, None, torch.zeros(4), torch.zeros(4))),
+        (ValueError, lambda: layer_norm_bwd(
+            x, x, None, torch.zeros(3), torch.zeros(4))),
+    ]
+    for err, call in cases:
+        with pytest.raises(err):
+            call()
+
+
+# ---------------------------------------------------------------- gated scan
+def scan_64(gate, x, h0, done, dhs=None, dhl=None):
+    """Values and bounds of hs, h_last (and dgate, dx, dh0) in 64 bits.
+
+    M and MD are the same recurrences on magnitudes: however a sum over time
+    is grouped, its partial sums stay below them. z, 1 - z and products of
+    them are off by at most 8 u for each step they span, each step's
+    arithmetic by 4 u more."""
+    dt = x.dtype
+    T, E, H = x.shape
+    g64 = gate.detach().double().cpu()
+    z, a, v = torch.sigmoid(g64), torch.sigmoid(-g64), x.detach().double().cpu()
+    h = torch.zeros(E, H).double() if h0 is None else h0.detach().double().cpu()
+    end = torch.zeros(T, E, dtype=torch.bool) if done is None \
+        else done.cpu() != 0
+    M, B = h.abs(), torch.zeros_like(h)
+    hs, bh, cs, ms, bs = [], [], [], [], []
+    for t in range(T):
+        cs.append(h), ms.append(M), bs.append(B)
+        h = a[t] * h + z[t] * v[t]
+        M = a[t] * M + z[t] * v[t].abs()
+        B = a[t] * B + 12 * U * M
+        hs.append(h), bh.append(B)
+        k = ~end[t].unsqueeze(-1)
+        h, M, B = (torch.where(k, q, torch.zeros_like(q)) for q in (h, M, B))
+    out = {"h_last": (h, half_step(h, F32) + B)}
+    if T:
+        hs, bh = torch.stack(hs), torch.stack(bh)
+        out["hs"] = (hs, half_step(hs, dt) + bh)
+    if dhs is not None or dhl is not None:
+        D = torch.zeros(E, H).double() if dhl is None else dhl.double().cpu()
+        MD, BD = D.abs(), torch.zeros_like(D)
+        dg, dx, tg, tx = ([None] * T for _ in range(4))
+        for t in range(T - 1, -1, -1):
+            k = ~end[t].unsqueeze(-1)
+            D, MD, BD = (torch.where(k, q, torch.zeros_like(q))
+                         for q in (D, MD, BD))
+            if dhs is not None:
+                D = D + dhs[t].double().cpu()
+                MD = MD + dhs[t].double().cpu().abs()
+            BD = BD + 4 * U * MD
+            dx[t] = z[t] * D
+            tx[t] = z[t] * (BD + 8 * U * MD)
+            dg[t] = D * (v[t] - cs[t]) * z[t] * a[t]
+            size = v[t].abs() + ms[t]
+            tg[t] = z[t] * a[t] * ((BD + 20 * U * MD) * size
+                                   + MD * (bs[t] + U * size))
+            D, MD = a[t] * D, a[t] * MD
+            BD = a[t] * BD + 8 * U * MD
+        dg, dx, tg, tx = (torch.stack(q) for q in (dg, dx, tg, tx))
+        out["dgate"] = (dg, half_step(dg, dt) + tg)
+        out["dx"] = (dx, half_step(dx, dt) + tx)
+        out["dh0"] = (D, half_step(D, F32) + BD)
+    return out
+
+
+def scan_inputs(seed, T, E, H, dtype, device, ends=0.1):
+    g = gen(seed)
+    gate = randn(g, T, E, H, dtype=dtype, device=device, scale=2, shift=-0.5)
+    x = randn(g, T, E, H, dtype=dtype, device=device)
+    h0 = randn(g, E, H, device=device)
+    done = (torch.rand(T, E, generator=g) < ends).to(torch.uint8).to(device)
+    dhs = randn(g, T, E, H, dtype=dtype, device=device)
+    dhl = randn(g, E, H, device=device)
+    return gate, x, h0, done, dhs, dhl
+
+
+def run_scan(gate, x, h0, done, dhs, dhl):
+    leaves = [t.detach().requires_grad_(True) for t in (gate, x, h0)
+              if t is not None]
+    hs, hl = gated_scan(*leaves[:2], leaves[2] if h0 is not None else None,
+                        done)
+    outs = [(o, d) for o, d in ((hs, dhs), (hl, dhl)) if d is not None]
+    grads = torch.autograd.grad([o for o, _ in outs], leaves,
+                                [d for _, d in outs])
+    return {"hs": hs, "h_last": hl, "dgate": grads[0], "dx": grads[1],
+            **({"dh0": grads[2]} if h0 is not None else {})}
+
+
+SCAN_SIZES = [(1, 1, 1), (1, 5, 64), (2, 3, 7), (5, 2, 130), (16, 4, 64),
+              (17, 3, 72), (63, 2, 33), (64, 3, 256), (65, 2, 64),
+              (100, 1, 1000), (129, 5, 40), (256, 1, 8), (300, 2, 66),
+              (1025, 1, 64), (2500, 1, 3), (4100, 2, 20)]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("T,E,H", SCAN_SIZES)
+def test_scan(device, dtype, T, E, H):
+    inputs = scan_inputs(T * 7 + E + H, T, E, H, dtype, device)
+    got = run_scan(*inputs)
+    want = scan_64(*inputs)
+    for name in got:
+        close(got[name], *want[name], f"{name} {T}x{E}x{H} {dtype}")
+    with torch.no_grad():
+        hs, hl = gated_scan(*inputs[:4])
+    assert torch.equal(hs, got["hs"]) and torch.equal(hl, got["h_last"])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("T,E,H", [(70, 2, 24), (1500, 1, 24), (3, 300, 70)])
+def test_scan_optional_inputs(device, T, E, H):
+    gate, x, h0, done, dhs, dhl = scan_inputs(9, T, E, H, F32, device)
+    for a in ((None, None, dhs, None), (h0, None, dhs, dhl),
+              (None, done, None, dhl), (h0, done.bool(), dhs, None)):
+        got, want = run_scan(gate, x, *a), scan_64(gate, x, *a)
+        for name in got:
+            close(got[name], *want[name], name)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+def test_scan_layouts(device, dtype):
+    """Halves of one projection, [E, T, H] data seen time-major, misaligned
+    bases, and broadcast inputs and gradients."""
+    g = gen(11)
+    T, E, H = 75, 3, 48
+    proj = randn(g, T, E, 2 * H, dtype=dtype, device=device)
+    odd = randn(g, T, E, 2 * H + 3, dtype=dtype, device=device)
+    batch = randn(g, E, T, 2 * H, dtype=dtype, device=device)
+    flip = randn(g, T, H, E, dtype=dtype, device=device).transpose(1, 2)
+    h0 = randn(g, H, E, device=device).t()
+    done = (torch.rand(E, T, generator=g) < 0.1).to(device).t()
+    dhs = randn(g, 1, E, 1, dtype=dtype, device=device).expand(T, E, H)
+    pairs = [proj.chunk(2, -1), (odd[..., 1:H + 1], odd[..., H + 2:-1]),
+             [q.transpose(0, 1) for q in batch.chunk(2, -1)], (flip, flip),
+             (proj[:, :1, :H].expand(T, E, H), odd[..., :H])]
+    for k, (gate, x) in enumerate(pairs):
+        got = run_scan(gate, x, h0, done, dhs, None)
+        want = scan_64(gate, x, h0, done, dhs, None)
+        for name in got:
+            close(got[name], *want[name], f"{name} of pair {k}")
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("T,E,H", [(90, 3, 40), (1700, 1, 40), (200, 64, 64)])
+def test_scan_reset_hides_what_came_before(device, T, E, H):
+    gate, x, h0, _, dhs, dhl = scan_inputs(13, T, E, H, F32, device)
+    cut = T - 41
+    done = torch.zeros(T, E, dtype=torch.uint8, device=device)
+    done[cut] = 1
+    clean = run_scan(gate, x, h0, done, dhs, dhl)
+    x2, h2 = x.clone(), h0.clone()
+    x2[3, :, 5] = math.nan
+    x2[7, :, 6] = math.inf
+    h2[:, 7] = math.nan
+    got = run_scan(gate, x2, h2, done, dhs, dhl)
+    for name in ("hs", "dgate", "dx"):
+        assert torch.equal(got[name][cut + 1:], clean[name][cut + 1:]), name
+    assert torch.equal(got["h_last"], clean["h_last"])
+    for col in (5, 6, 7):  # and it is not hidden before
+        assert not got["hs"][7:cut + 1, :, col].isfinite().any()
+    # gradients do not pass an end either
+    d2 = dhs.clone()
+    d2[cut + 1:] = math.nan
+    late = run_scan(gate, x, h0, done, d2, dhl)
+    assert torch.equal(late["dx"][:cut + 1], clean["dx"][:cut + 1])
+    assert torch.equal(late["dh0"], clean["dh0"])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_scan_edges(device):
+    h0 = torch.randn(2, 6).to(device).requires_grad_(True)
+    x = torch.zeros(0, 2, 6, device=device, requires_grad=True)
+    hs, hl = gated_scan(x, x, h0)
+    assert hs.shape == (0, 2, 6) and torch.equal(hl, h0)
+    dh, = torch.autograd.grad(hl.sum(), h0)
+    assert torch.equal(dh, torch.ones_like(dh))
+    for shape in ((4, 0, 6), (4, 2, 0)):
+        hs, hl = gated_scan(torch.zeros(shape, device=device),
+                            torch.zeros(shape, device=device))
+        assert hs.shape == shape and hl.shape == shape[1:]
+    # saturated gates: held for good, or replaced at once
+    inf = torch.full((5, 2, 6), math.inf, device=device)
+    v = torch.randn(5, 2, 6).to(device)
+    hs, hl = gated_scan(-inf, v, h0.detach())
+    assert torch.equal(hs, h0.detach().expand(5, 2, 6))
+    hs, hl = gated_scan(inf, v, h0.detach())
+    assert torch.equal(hs, v) and torch.equal(hl, v[-1])
+    big = torch.full((5, 2, 6), 200.0, device=device)
+    assert torch.equal(gated_scan(big, v, h0.detach())[0], v)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("E,H", [(1, 1), (3, 7), (64, 256), (33, 100)])
+def test_scan_step(device, dtype, E, H):
+    """Steps with the carry in place are the sequence."""
+    T = 6
+    gate, x, h0, done, _, _ = scan_inputs(17, T, E, H, dtype, device, 0.3)
+    want = scan_64(gate, x, h0, done)
+    h = h0.clone()
+    prev = None
+    for t in range(T):
+        out = gated_scan_step(gate[t], x[t], h, prev)
+        assert out.dtype == dtype
+        close(out, want["hs"][0][t], want["hs"][1][t], f"step {t}")
+        prev = done[t]
+    h.masked_fill_(prev.bool().unsqueeze(-1), 0.0)
+    close(h, *want["h_last"], "state")
+
+
+def test_scan_refusals():
+    x, h = torch.zeros(4, 2, 6), torch.zeros(2, 6)
+    d = torch.zeros(4, 2, dtype=torch.uint8)
+    st = torch.zeros(1, 2, 6)
+    cases = [
+        (ValueError, lambda: gated_scan_fwd(x, torch.zeros(4, 2, 5))),
+        (ValueError, lambda: gated_scan_fwd(x.half(), x)),
+        (ValueError, lambda: gated_scan_fwd(x[0], x[0])),
+        (TypeError, lambda: gated_scan_fwd(x.double(), x.double())),
+        (ValueError, lambda: gated_scan_fwd(x, x, h.half())),
+        (ValueError, lambda: gated_scan_fwd(x, x, torch.zeros(2, 5))),
+        (ValueError, lambda: gated_scan_fwd(x, x, h, d.float())),
+        (ValueError, lambda: gated_scan_fwd(x, x, h, d.t())),
+        (ValueError, lambda: gated_scan_fwd(x, x, h.to("meta"))),
+        (ValueError, lambda: gated_scan_fwd(
+            torch.zeros(1, device="meta").expand(1, 1 << 16, 1 << 15),
+            torch.zeros(1, device="meta").expand(1, 1 << 16, 1 << 15))),
+        (ValueError, lambda: gated_scan_bwd(x.half(), h, x, x, st)),
+        (ValueError, lambda: gated_scan_bwd(x, h[:1], x, x, st)),
+        (ValueError, lambda: gated_scan_bwd(x, h, x, x, st[:0])),
+        (ValueError, lambda: gated_scan_step(x[0], x[0], h.t())),
+        (ValueError, lambda: gated_scan_step(
+            x[0], x[0], torch.zeros(2, 12)[:, ::2])),
+    ]
+    for err, call in cases:
+        with pytest.raises(err):
+            call()
+
+
+# -------------------------------------------------------- log probabilities
+def logp_64(logits, actions, mask, top_k=0, dlogp=None, dent=None):
+    """Values and bounds in 64 bits. p_j is off by its exponent's roundings,
+    (|x_j - m| + |log s|) u each, and the sum's L u."""
+    dt = logits.dtype
+    A = logits.shape[-1]
+    x = logits.detach().double().cpu().reshape(-1, A)
+    act = actions.cpu().reshape(-1)
+    n = x.shape[0]
+    ok = x != -math.inf
+    if mask is not None:
+        ok &= mask.cpu().reshape(-1, A) != 0
+    L = (32 + A / 64) * U
+    o = {k: torch.zeros(n).double() for k in ("logp", "entropy", "tl", "th")}
+    top = torch.full((n, top_k), -math.inf).double()
+    ttop, tix = torch.zeros(n, top_k).double(), torch.full((n, top_k), -1)
+    grad, tgrad = torch.zeros(n, A).double(), torch.zeros(n, A).double()
+    for i in range(n):
+        j = ok[i].nonzero().squeeze(-1)
+        a = int(act[i])
+        if not len(j):
+            o["logp"][i] = 0.0 if a < 0 else -math.inf
+            continue
+        v = x[i, j]
+        if not (v < math.inf).all():  # NaN or +inf among the allowed
+            o["logp"][i] = 0.0 if a < 0 else math.nan
+            o["entropy"][i] = math.nan
+            top[i] = math.nan
+            grad[i, j] = math.nan
+            continue
+        m = v.max()
+        d = v - m
+        s = d.exp().sum()
+        lp = d - s.log()
+        p = lp.exp()
+        H = -(p * torch.where(p > 0, lp, torch.zeros_like(lp))).sum()
+        dd = torch.where(p > 0, d.abs(), torch.zeros_like(d))
+        dls = L + 4 * U + U * (p * (2 * dd + 4)).sum()  # log s, absolute
+        tlp = dls + 4 * U * (d.abs() + s.log().abs())  # (x - m) - log s
+        o["entropy"][i] = H
+        o["th"][i] = dls + 2 * U * (s.log() + H) + (
+            p * dd * (L + 8 * U + 4 * U * dd)).sum() + dls * (p * dd).sum()
+        hit = (j == a).nonzero().squeeze(-1)
+        if a >= 0:
+            o["logp"][i] = lp[hit[0]] if len(hit) else -math.inf
+            o["tl"][i] = tlp[hit[0]] if len(hit) else 0.0
+        order = torch.argsort(-v, stable=True)[:top_k]
+        top[i, :len(order)] = lp[order]
+        ttop[i, :len(order)] = tlp[order]
+        tix[i, :len(order)] = j[order]
+        if dlogp is not None or dent is not None:
+            dl = float(dlogp.reshape(-1)[i]) if dlogp is not None else 0.0
+            dh = float(dent.reshape(-1)[i]) if dent is not None else 0.0
+            dl = dl if len(hit) else 0.0
+            lz = torch.where(p > 0, lp, torch.zeros_like(lp))
+            e = p * (dls + 8 * U * (lz.abs() + s.log().abs() + 1))
+            w = torch.zeros_like(p)
+            w[hit] = 1.0
+            grad[i, j] = dl * (w - p) - dh * p * (lz + H)
+            tgrad[i, j] = abs(dl) * (e + 2 * U * (w + p)) + abs(dh) * (
+                (e + 4 * U * p) * (lz.abs() + H)
+                + p * (torch.where(p > 0, tlp, 0.0) + o["th"][i]))
+    out = {"logp": (o["logp"], o["tl"] + half_step(o["logp"], F32)),
+           "entropy": (o["entropy"], o["th"] + half_step(o["entropy"], F32)),
+           "dlogits": (grad, tgrad + half_step(grad, dt))}
+    for k in ("logp", "entropy"):
+        out[k] = tuple(t.nan_to_num(nan=0.0, posinf=0.0, neginf=0.0) if q
+                       else t for q, t in enumerate(out[k]))
+    if top_k:
+        out["top_logp"] = (top, ttop + half_step(
+            top, F32).nan_to_num(nan=0.0, posinf=0.0, neginf=0.0))
+        out["top_index"] = tix
+    return out
+
+
+def check_logp(logits, actions, mask, top_k, dlogp, dent, what=""):
+    x = logits.detach().requires_grad_(True)
+    r = action_logprobs(x, actions, mask, top_k=top_k)
+    outs = [(o, d) for o, d in ((r.logp, dlogp), (r.entropy, dent))
+            if d is not None]
+    dx, = torch.autograd.grad([o for o, _ in outs], x, [d for _, d in outs])
+    assert dx.dtype == logits.dtype and dx.shape == logits.shape
+    A = logits.shape[-1]
+    want = logp_64(logits, actions, mask, top_k, dlogp, dent)
+    close(r.logp.reshape(-1), *want["logp"], f"logp {what}")
+    close(r.entropy.reshape(-1), *want["entropy"], f"entropy {what}")
+    close(dx.reshape(-1, A), *want["dlogits"], f"dlogits {what}")
+    if top_k:
+        got = r.top_index.cpu().reshape(-1, top_k)
+        assert torch.equal(got, want["top_index"]), f"top_index {what}"
+        close(r.top_logp.reshape(-1, top_k), *want["top_logp"],
+              f"top_logp {what}")
+    else:
+        assert r.top_logp is None and r.top_index is None
+    with torch.no_grad():
+        q = action_logprobs(logits, actions, mask, top_k=top_k)
+    for a, b in zip(q, r):
+        assert a is b is None or torch.equal(a.nan_to_num(7.0),
+                                             b.detach().nan_to_num(7.0))
+
+
+LOGP_SIZES = [(1, 1), (3, 2), (50, 5), (300, 17), (5, 21), (70, 64), (33, 65),
+              (9, 100), (4, 256), (7, 1000), (3, 1024), (5, 4097), (2, 8192),
+              (2, 10007), (1, 20000), (1, 70000), (3, 32768)]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,A", LOGP_SIZES)
+def test_logp(device, dtype, rows, A):
+    g = gen(rows + A * 3)
+    for masked, k in ((False, 0), (True, min(A, 20)), (False, min(A, 5)),
+                      (True, min(A, 64))):
+        x = randn(g, rows, A, dtype=dtype, device=device, scale=2.0)
+        act = torch.randint(0, A, (rows,), generator=g).to(device)
+        act[rows // 2] = -1 if rows > 1 else act[0]
+        mask = None
+        if masked:
+            mask = torch.rand(rows, A, generator=g) < 0.6
+            mask[rows // 3] = rows == 1
+            mask = mask.to(device)
+            mask = mask if k % 2 else mask.to(torch.uint8)
+        dl, dh = (randn(g, rows, device=device) for _ in range(2))
+        check_logp(x, act, mask, k, dl, dh, f"{rows}x{A} {dtype} {masked} {k}")
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("A", [17, 200, 9000])
+def test_logp_one_gradient_alone(device, A):
+    g = gen(A)
+    x = randn(g, 6, A, device=device)
+    act = torch.randint(0, A, (6,), generator=g).to(device)
+    d = randn(g, 6, device=device)
+    check_logp(x, act, None, 0, d, None)
+    check_logp(x, act, None, 3, None, d)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("A", [7, 30, 150, 1003, 9000, 40000])
+def test_logp_hard_rows(device, dtype, A):
+    """Rows of the values that masks, padding and broken models bring."""
+    low = torch.finfo(dtype).min
+    g = gen(A)
+    x = randn(g, 14, A, dtype=dtype)
+    mask = torch.ones(14, A, dtype=torch.uint8)
+    act = torch.randint(0, A, (14,), generator=g)
+    x[0] = low                       # everything at the lowest value
+    x[1, 1:] = low                   # one above it
+    x[2] = -math.inf                 # nothing has a probability
+    x[3, ::2] = -math.inf            # what has none is not an alternative
+    act[3] = 0
+    x[4, 3] = math.nan               # NaN and inf in masked places
+    x[4, 4] = math.inf
+    mask[4, 3:5] = 0
+    act[4] = 4
+    x[5, 2] = math.nan               # in allowed ones
+    x[6, 2] = math.inf
+    act[7] = A                       # beyond the last action
+    mask[8] = 0                      # a mask that leaves nothing
+    act[9] = -100
+    x[10] = 1.0                      # ties: lowest index first
+    mask[10, 1] = 0
+    x[11] = torch.sort(x[11].float()).values.to(dtype)  # ever better ones
+    x[12] = 0.0
+    x[12, 1::2] = -0.0               # which are equal
+    mask[13] = 0
+    mask[13, A - 1] = 1              # the last one alone
+    act[13] = A - 1
+    dl, dh = (randn(g, 14, device=device) for _ in range(2))
+    check_logp(x.to(device), act.to(device), mask.to(device), min(A, 9), dl,
+               dh, f"{A} {dtype}")
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("A", [19, 120, 5000])
+def test_logp_layouts(device, dtype, A):
+    g = gen(A + 1)
+    wide = randn(g, 5, 3, A + 9, dtype=dtype, device=device)
+    wmask = (torch.rand(5, 3, A + 5, generator=g) < 0.7).to(device)
+    flat = randn(g, 15 * A + 1, dtype=dtype, device=device)
+    act = torch.randint(0, A, (3, 5), generator=g).to(device).t()
+    one = torch.ones(1, 1, device=device)
+    for k, x in enumerate((wide[..., :A], wide[..., 1:A + 1],
+                           flat[1:].view(5, 3, A),
+                           wide[:, :, 8:A + 8].transpose(0, 1),
+                           wide[:1, :, :A].expand(5, 3, A),
+                           randn(g, 5, A, 3, dtype=dtype,
+                                 device=device).transpose(1, 2))):
+        lead = x.shape[:-1]
+        a = act if lead == (5, 3) else act.t()
+        m = wmask[..., 3:A + 3] if lead == (5, 3) else \
+            wmask[..., 3:A + 3].transpose(0, 1)
+        check_logp(x, a, m, 4, one.expand(lead), None, f"view {k}")
+    check_logp(wide[0, 0, :A], act[0, 0], wmask[0, 0, :A], 4, one[0, 0],
+               one[0, 0], "a single row")
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_logp_edges(device):
+    x = torch.zeros(0, 9, device=device, requires_grad=True)
+    r = action_logprobs(x, torch.zeros(0, dtype=torch.int64, device=device),
+                        top_k=2)
+    assert r.logp.shape == (0,) and r.top_index.shape == (0, 2)
+    dx, = torch.autograd.grad(r.logp.sum() + r.entropy.sum(), x)
+    assert dx.shape == (0, 9)
+    # outputs are the user's to change before the backward pass
+    x = torch.randn(4, 9).to(device).requires_grad_(True)
+    act = torch.tensor([1, 2, 3, 4], device=device)
+    r = action_logprobs(x, act, top_k=3)
+    want, = torch.autograd.grad(2 * r.logp.sum(), x, retain_graph=True)
+    r.logp.mul_(2)
+    r.top_logp.zero_()
+    got, = torch.autograd.grad(r.logp.sum(), x)
+    assert torch.equal(got, want)
+    assert not r.top_logp.requires_grad
+
+
+def test_logp_refusals():
+    x, a = torch.zeros(4, 8), torch.zeros(4, dtype=torch.int64)
+    cases = [
+        (ValueError, lambda: action_logprobs(torch.zeros(()), a)),
+        (ValueError, lambda: action_logprobs(torch.zeros(4, 0), a)),
+        (TypeError, lambda: action_logprobs(x.double(), a)),
+        (ValueError, lambda: action_logprobs(x, a[:3])),
+        (ValueError, lambda: action_logprobs(x, a.int())),
+        (ValueError, lambda: action_logprobs(x, a, torch.ones(4, 7).bool())),
+        (ValueError, lambda: action_logprobs(x, a, torch.ones(8).bool())),
+        (ValueError, lambda: action_logprobs(x, a, torch.ones(4, 8))),
+        (ValueError, lambda: action_logprobs(x, a, top_k=9)),
+        (ValueError, lambda: action_logprobs(x, a, top_k=-1)),
+        (ValueError, lambda: action_logprobs(
+            torch.zeros(4, 100), a, top_k=65)),
+        (ValueError, lambda: action_logprobs(x, a.to("meta"))),
+        (ValueError, lambda: action_logprobs_bwd(
+            a.float()[:2], None, x, a, None, x[:, :2].contiguous(),
+            a.float())),
+        (ValueError, lambda: action_logprobs_bwd(
+            a.float(), None, x, a, None, x[:3, :2].contiguous(), a.float())),
+    ]
+    for err, call in cases:
+        with pytest.raises(err):
+            call()
+
+
+# ------------------------------------------------------ gradients, together
+def test_reference_gradients_against_differences():
+    """The torch references in 64 bits against central differences."""
+    from rlgpuschedule_amd.ops.seq_ref import (action_logprobs_reference,
+                                               gated_scan_reference,
+                                               layer_norm_reference)
+    g = gen(21)
+
+    def r(*s):
+        return torch.randn(*s, generator=g).double().requires_grad_(True)
+
+    assert torch.autograd.gradcheck(
+        lambda x, w, b: layer_norm_reference(x, w, b), (r(3, 7), r(7), r(7)))
+    done = torch.rand(5, 2, generator=g) < 0.3
+    assert torch.autograd.gradcheck(
+        lambda a, b, h: gated_scan_reference(a, b, h, done),
+        (r(5, 2, 3), r(5, 2, 3), r(2, 3)))
+    mask = torch.rand(4, 6, generator=g) < 0.7
+    mask[2] = False
+    act = torch.tensor([1, 5, 0, -1])
+    mask[0, 1] = mask[1, 5] = True
+
+    def logps(x):
+        lp, h, _, _ = action_logprobs_reference(x, act, mask)
+        return lp[[0, 1, 3]], h
+
+    assert torch.autograd.gradcheck(logps, (r(4, 6),))
+
+
+def net(p, obs, done, h0, mask, act, dtype):
+    """The operators as a policy runs them, with torch between."""
+    T, E, _ = obs.shape
+    x = layer_norm(torch.tanh(obs @ p[0]), p[1], p[2])
+    gate, cand = (x @ p[3]).to(dtype).chunk(2, -1)
+    hs, hl = gated_scan(gate, cand, h0, done)
+    logits = hs @ p[4]
+    return action_logprobs(logits, act, mask), hl
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_run_together_against_differences(device):
+    """Norm, scan and log probabilities in one loss: the gradient along a
+    direction is the loss's difference along it, in 64 bits on the CPU."""
+    from rlgpuschedule_amd.ops.seq_ref import (action_logprobs_reference,
+                                               gated_scan_reference,
+                                               layer_norm_reference)
+    g = gen(23)
+    T, E, D, H, A = 70, 3, 12, 32, 17
+    obs = randn(g, T, E, D)
+    done = (torch.rand(T, E, generator=g) < 0.05).to(torch.uint8)
+    mask = torch.rand(T, E, A, generator=g) < 0.7
+    act = torch.randint(0, A, (T, E), generator=g)
+    mask.scatter_(-1, act.unsqueeze(-1), True)
+    h0 = randn(g, E, H)
+    wl, wh = randn(g, T, E), randn(g, T, E)
+    p0 = [randn(g, D, H, scale=0.4), randn(g, H, scale=0.2, shift=1.0),
+          randn(g, H, scale=0.2), randn(g, H, 2 * H, scale=0.3),
+          randn(g, H, A, scale=0.5)]
+
+    def loss64(p):
+        p = [t.double() for t in p]
+        x = layer_norm_reference(torch.tanh(obs.double() @ p[0]), p[1], p[2])
+        gate, cand = (x @ p[3]).chunk(2, -1)
+        hs, hl = gated_scan_reference(gate, cand, h0.double(), done)
+        lp, H_, _, _ = action_logprobs_reference(hs @ p[4], act, mask)
+        return (lp * wl).sum() + (H_ * wh).sum() + hl.sum()
+
+    p = [t.clone().to(device).requires_grad_(True) for t in p0]
+    r, hl = net(p, obs.to(device), done.to(device), h0.to(device),
+                mask.to(device), act.to(device), F32)
+    loss = (r.logp * wl.to(device)).sum() + (
+        r.entropy * wh.to(device)).sum() + hl.sum()
+    grads = [q.cpu().double() for q in torch.autograd.grad(loss, p)]
+    for trial in range(3):
+        v = [torch.randn(t.shape, generator=g).double() for t in p0]
+        step = 1e-6
+        up = loss64([t.double() + step * d for t, d in zip(p0, v)])
+        down = loss64([t.double() - step * d for t, d in zip(p0, v)])
+        slope = float(up - down) / (2 * step)
+        got = sum(float((a * d).sum()) for a, d in zip(grads, v))
+        size = sum(float((a * d).abs().sum()) for a, d in zip(grads, v))
+        # the products between the operators are sums of up to T E terms in
+        # 32 bits: 512 u of the terms' magnitudes, and the difference's own
+        # 1e-6 relative
+        assert abs(got - slope) <= 512 * U * size + 1e-6 * abs(slope) + 1e-5
+
+
+# ------------------------------------------------ streams, graphs, far ends
+def all_calls(seed, small=True):
+    """Inputs of every entry point on the GPU and a function of them."""
+    g = gen(seed)
+    T, E, H, A = (70, 3, 40, 130) if small else (600, 9, 200, 9000)
+    t = {"x": randn(g, T * E, H, device="cuda"),
+         "w": randn(g, H, device="cuda"), "b": randn(g, H, device="cuda"),
+         "dy": randn(g, T * E, H, device="cuda"),
+         "gate": randn(g, T, E, H, device="cuda"),
+         "h0": randn(g, E, H, device="cuda"),
+         "done": (torch.rand(T, E, generator=g) < 0.1).cuda(),
+         "logits": randn(g, T * E, A, device="cuda"),
+         "act": torch.randint(0, A, (T * E,), generator=g).cuda(),
+         "mask": (torch.rand(T * E, A, generator=g) < 0.5).cuda(),
+         "d": randn(g, T * E, device="cuda")}
+
+    def run():
+        y, mean, rstd = layer_norm_fwd(t["x"], t["w"], t["b"])
+        dx, dw, db = layer_norm_bwd(t["dy"], t["x"], t["w"], mean, rstd)
+        v = y.view(T, E, H)
+        hs, hl, st = gated_scan_fwd(t["gate"], v, t["h0"], t["done"])
+        dg, dv, dh0 = gated_scan_bwd(dx.view(T, E, H), hl, t["gate"], v, st,
+                                     t["done"])
+        h = t["h0"].clone()
+        o = gated_scan_step(t["gate"][0], v[0], h, t["done"][0])
+        lp, H_, st2, tl, ti = action_logprobs_fwd(t["logits"], t["act"],
+                                                  t["mask"], 7)
+        dl = action_logprobs_bwd(t["d"], lp.nan_to_num(0.0, 0.0, 0.0),
+                                 t["logits"], t["act"], t["mask"], st2, H_)
+        return [y, dx, dw, db, hs, hl, dg, dv, dh0, h, o, lp, H_, tl, ti, dl]
+
+    return t, run
+
+
+def same(a, b):
+    return all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("small", [True, False])
+def test_graph_replays_and_eager_between(small):
+    """Two captured graphs, replayed in turn with new inputs and eager calls
+    between, give the eager results each time."""
+    made = [all_calls(31, small), all_calls(32, small)]
+    graphs = []
+    for t, run in made:
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            run()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = run()
+        graphs.append((graph, out))
+    for k in range(3):
+        for (t, run), (graph, out) in zip(made, graphs):
+            for q in t.values():
+                if q.dtype == F32:
+                    q.mul_(0.9).add_(0.01 * k)
+            want = [q.clone() for q in run()]
+            graph.replay()
+            torch.cuda.synchronize()
+            assert same(out, want), f"replay {k}"
+        both = [run for _, run in made][k % 2]()
+        assert same(both, graphs[k % 2][1])
+
+
+@pytest.mark.gpu
+def test_streams_and_repeats():
+    """Calls on streams of their own, at once, give the default stream's
+    bits, every time."""
+    made = [all_calls(s, False) for s in (41, 42, 43)]
+    want = [[q.clone() for q in run()] for _, run in made]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in made]
+    for _ in range(4):
+        got = []
+        for s, (_, run) in zip(streams, made):
+            with torch.cuda.stream(s):
+                got.append(run())
+        torch.cuda.synchronize()
+        assert all(same(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
+def test_captured_autograd_and_its_refusal():
+    """A training pass through autograd can be captured; where an eager graph
+    of the same leaves is alive it is refused, and afterwards works."""
+    w = torch.ones(16, device="cuda", requires_grad=True)
+    x = torch.randn(5, 16, device="cuda")
+    eager = layer_norm(x, w)
+    with pytest.raises(RuntimeError, match="alive"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            layer_norm(x, w)
+    want, = torch.autograd.grad(eager.square().sum(), w)
+    del eager
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.autograd.grad(layer_norm(x, w).square().sum(), w)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got, = torch.autograd.grad(layer_norm(x, w).square().sum(), w)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits():
+    """Rows whose elements lie past 2^31 are read and written there."""
+    dev = "cuda"
+    rows, D = (1 << 20) + 5, 2056
+    x = torch.empty(rows, D, dtype=BF16, device=dev).normal_()
+    y, mean, rstd = layer_norm_fwd(x)
+    dx, _, _ = layer_norm_bwd(x, x, None, mean, rstd,
+                              needs=(True, False, False))
+    want = norm_64(x[-4:], None, None, 1e-5, x[-4:])
+    close(y[-4:], *want["y"], "y")
+    close(dx[-4:], *want["dx"], "dx")
+    del y, dx
+    A = 65544
+    z = x.view(-1)[:32800 * A].view(32800, A)
+    act = torch.randint(0, A, (32800,), device=dev)
+    lp, H, st2, tl, ti = action_logprobs_fwd(z, act, None, 4)
+    d = torch.ones_like(lp)
+    dz = action_logprobs_bwd(d, d, z, act, None, st2, H)
+    want = logp_64(z[-2:], act[-2:], None, 4, d[-2:], d[-2:])
+    close(lp[-2:], *want["logp"], "logp")
+    close(H[-2:], *want["entropy"], "entropy")
+    close(dz[-2:], *want["dlogits"], "dlogits")
+    assert torch.equal(ti[-2:].cpu(), want["top_index"])
+    del dz, z
+    T, E, H_ = 70, 8192, 4096
+    v = x.view(-1)[:T * E // 2 * H_ * 1].view(T // 2, E, H_)
+    gate = x.view(-1)[1:1 + v.numel()].view(v.shape)
+    v = v.repeat(2, 1, 1)
+    gate = gate.repeat(2, 1, 1)
+    hs, hl, st = gated_scan_fwd(gate, v)
+    dg, dv, _ = gated_scan_bwd(v, None, gate, v, st)
+    cut = (slice(None), slice(-1, None), slice(-40, None))
+    want = scan_64(gate[cut], v[cut], None, None, v[cut])
+    close(hs[cut], *want["hs"], "hs")
+    close(hl[cut[1:]], *want["h_last"], "h_last")
+    close(dg[cut], *want["dgate"], "dgate")
+    close(dv[cut], *want["dx"], "dx")
