@@ -10,6 +10,7 @@
 // not even a NaN, is seen after it. The state is held in 32 bits throughout;
 // the backward pass does not read the rounded hs but computes c again from
 // the 32-bit states kept at every kKeep-th step.
+#include "seq_api.h"
 #include "seq_common.h"
 
 namespace {

@@ -7,6 +7,7 @@
 //
 // Statistics and sums are held in 32 bits; y, dx, dw and db are rounded to
 // their types once.
+#include "seq_api.h"
 #include "seq_common.h"
 
 namespace {

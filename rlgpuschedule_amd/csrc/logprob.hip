@@ -9,6 +9,7 @@
 // probability 0, no gradient, never an alternative. Sums are held in 32 bits;
 // m and log s are kept apart: where every logit is the type's lowest value,
 // their sum would lose log s.
+#include "seq_api.h"
 #include "seq_common.h"
 
 namespace {
@@ -20,7 +21,7 @@ struct LogpFwd {
   const uint8_t* mask;  // null: all allowed
   float* logp;
   float* entropy;
-  float* stats;  // [rows, 2]: m, log s
+  float* stats;  // [rows, 3]: m, log s, H; or null
   float* top_logp;     // [rows, k]
   int64_t* top_index;  // [rows, k]
   int64_t rows, A, x_stride, mask_stride;
@@ -34,7 +35,6 @@ struct LogpBwd {
   const int64_t* actions;
   const uint8_t* mask;
   const float* stats;
-  const float* entropy;
   void* dlogits;
   int64_t rows, A, x_stride, mask_stride;
 };
@@ -104,9 +104,13 @@ __global__ __launch_bounds__(256) void logp_fwd_kernel(LogpFwd p) {
     if (some && a < p.A && a >= 0 && !(ok && !ok[a]))
       lp = (float)x[a] - q.m - ls;
     p.logp[row] = a < 0 ? 0.f : lp;
-    p.entropy[row] = broken ? NAN : some ? ls - q.u / q.s : 0.f;
-    p.stats[2 * row] = broken ? NAN : some ? q.m : 0.f;
-    p.stats[2 * row + 1] = broken ? NAN : some ? ls : 0.f;
+    const float H = broken ? NAN : some ? ls - q.u / q.s : 0.f;
+    p.entropy[row] = H;
+    if (p.stats) {
+      p.stats[3 * row] = broken ? NAN : some ? q.m : 0.f;
+      p.stats[3 * row + 1] = broken ? NAN : some ? ls : 0.f;
+      p.stats[3 * row + 2] = H;
+    }
   }
   uint64_t last = ~0ull;
   for (int j = 0; j < p.k; ++j) {
@@ -144,8 +148,8 @@ __global__ __launch_bounds__(256) void logp_bwd_kernel(LogpBwd p) {
   const uint8_t* ok = p.mask ? p.mask + row * p.mask_stride : nullptr;
   T* out = (T*)p.dlogits + row * p.A;
   const int64_t act = p.actions[row];
-  const float m = p.stats[2 * row], ls = p.stats[2 * row + 1];
-  const float H = p.entropy[row];
+  const float m = p.stats[3 * row], ls = p.stats[3 * row + 1];
+  const float H = p.stats[3 * row + 2];
   float dl = p.dlogp ? p.dlogp[row] : 0.f;
   const float dh = p.dentropy ? p.dentropy[row] : 0.f;
   // a taken action of probability 0 is a constant -inf
@@ -199,14 +203,13 @@ extern "C" int rlsched_logp_fwd(int device, void* stream, const void* logits,
 extern "C" int rlsched_logp_bwd(int device, void* stream, const float* dlogp,
                                 const float* dentropy, const void* logits,
                                 const int64_t* actions, const uint8_t* mask,
-                                const float* stats, const float* entropy,
-                                void* dlogits, int64_t rows, int64_t A,
-                                int64_t x_stride, int64_t mask_stride,
-                                int type) {
+                                const float* stats, void* dlogits,
+                                int64_t rows, int64_t A, int64_t x_stride,
+                                int64_t mask_stride, int type) {
   OnDevice on(device);
   if (on.err != hipSuccess) return on.err;
-  const LogpBwd p = {dlogp, dentropy, logits,  actions, mask,     stats,
-                     entropy, dlogits, rows, A, x_stride, mask_stride};
+  const LogpBwd p = {dlogp, dentropy, logits, actions,  mask,       stats,
+                     dlogits, rows,   A,      x_stride, mask_stride};
   const hipStream_t s = (hipStream_t)stream;
   if (type == F32) return bwd<float>(p, s);
   if (type == BF16) return bwd<bf16>(p, s);

@@ -14,6 +14,7 @@ CSRC = PKG / "csrc"
 OUT = PKG / "ops"
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
+CXX = os.environ.get("CXX", "g++")
 ARCH = os.environ.get("RLS_OFFLOAD_ARCH", "gfx950")
 
 # Packed FP32 instructions stay off: hipcc -O3 forms them from ordinary float
@@ -32,7 +33,35 @@ _LIBS = {
     "librlsched_norm.so": ["layer_norm.hip"],
     "librlsched_scan.so": ["gated_scan.hip"],
     "librlsched_logp.so": ["logprob.hip"],
+    "librlsched_seq.so": ["seq_bind.cpp"],
 }
+
+# torch bindings: host code, linked with the kernel libraries beside them
+_BINDS = {
+    "librlsched_seq.so": ["librlsched_norm.so", "librlsched_scan.so",
+                          "librlsched_logp.so"],
+}
+
+
+def _bind_flags(name: str) -> list[str]:
+    import sysconfig
+
+    import torch
+    root = Path(torch.__file__).resolve().parent
+    rocm = Path(HIPCC).resolve().parent.parent
+    abi = int(torch.compiled_with_cxx11_abi())
+    return (["-O2", "-std=c++17", "-fPIC", "-shared",
+             "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+             f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
+             f"-I{sysconfig.get_paths()['include']}"]
+            + [f"-isystem{d}" for d in
+               (root / "include", root / "include/torch/csrc/api/include",
+                rocm / "include")]
+            + [f"-L{root / 'lib'}", f"-L{OUT}", "-Wl,-rpath,$ORIGIN",
+               "-Wl,--no-as-needed"]
+            + [f"-l:{lib}" for lib in _BINDS[name]]
+            + ["-ltorch", "-ltorch_cpu", "-ltorch_hip", "-lc10", "-lc10_hip",
+               "-ltorch_python"])
 
 
 def source_hash(name: str) -> str:
@@ -42,6 +71,9 @@ def source_hash(name: str) -> str:
     kernels."""
     import hashlib
     h = hashlib.sha256(" ".join(FLAGS).encode())
+    if name in _BINDS:
+        import torch
+        h.update(torch.__version__.encode())
     srcs = [CSRC / s for s in _LIBS[name]] + sorted(CSRC.glob("*.h"))
     for p in sorted(srcs):
         h.update(p.name.encode())
@@ -78,16 +110,20 @@ def build_lib(name: str, verbose: bool = False, force: bool = False) -> Path:
         return so
     h = source_hash(name)
     tmp = so.with_suffix(f".{os.getpid()}.tmp")   # replaced whole, when done
-    cmd = [
-        HIPCC, f"--offload-arch={ARCH}", *FLAGS,
-        f'-DRLS_SOURCE_HASH="{h}"', "-o", str(tmp),
-    ] + [str(s) for s in srcs]
+    head = ([CXX] if name in _BINDS
+            else [HIPCC, f"--offload-arch={ARCH}", *FLAGS])
+    cmd = [*head, f'-DRLS_SOURCE_HASH="{h}"', "-o", str(tmp),
+           *(str(s) for s in srcs)]
+    if name in _BINDS:
+        for lib in _BINDS[name]:
+            build_lib(lib, verbose)
+        cmd += _bind_flags(name)
     if verbose:
         print("+", " ".join(cmd))
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         tmp.unlink(missing_ok=True)
-        raise RuntimeError(f"hipcc failed for {name}:\n{r.stdout}\n{r.stderr}")
+        raise RuntimeError(f"{cmd[0]} failed for {name}:\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, so)
     got = embedded_hash(so)
     if got != h:
@@ -118,12 +154,14 @@ def verify_loaded(lib, name: str) -> None:
 
 def build_all(verbose: bool = False, force: bool = False) -> list[Path]:
     """Build every library (force: also those whose binary is current),
-    a few compilers at a time."""
+    a few compilers at a time, and then the bindings linked with them."""
     from concurrent.futures import ThreadPoolExecutor
     names = [name for name, srcs in _LIBS.items()
              if all((CSRC / s).exists() for s in srcs)]
+    kernels = [n for n in names if n not in _BINDS]
     with ThreadPoolExecutor(max_workers=4) as pool:
-        return list(pool.map(lambda n: build_lib(n, verbose, force), names))
+        out = list(pool.map(lambda n: build_lib(n, verbose, force), kernels))
+    return out + [build_lib(n, verbose, force) for n in names if n in _BINDS]
 
 
 if __name__ == "__main__":

@@ -12,6 +12,7 @@ import torch
 
 from rlgpuschedule_amd import (action_logprobs, gated_scan, gated_scan_step,
                                layer_norm)
+from rlgpuschedule_amd.ops._seq import ext
 from rlgpuschedule_amd.ops.logprob import (action_logprobs_bwd,
                                            action_logprobs_fwd)
 from rlgpuschedule_amd.ops.norm import layer_norm_bwd, layer_norm_fwd
@@ -218,6 +219,11 @@ def test_norm_refusals():
             x.half(), x, None, torch.zeros(4), torch.zeros(4))),
         (ValueError, lambda: layer_norm_bwd(
             x, x, None, torch.zeros(3), torch.zeros(4))),
+        (TypeError, lambda: layer_norm_bwd(
+            x, x, None, torch.zeros(4), torch.zeros(4), torch.float16)),
+        (ValueError, lambda: layer_norm_bwd(
+            x, x, None, torch.zeros(4), torch.zeros(4))),
+        (ValueError, lambda: layer_norm_fwd(x)),  # not on a GPU
     ]
     for err, call in cases:
         with pytest.raises(err):
@@ -446,7 +452,12 @@ def test_scan_refusals():
         (ValueError, lambda: gated_scan_bwd(x.half(), h, x, x, st)),
         (ValueError, lambda: gated_scan_bwd(x, h[:1], x, x, st)),
         (ValueError, lambda: gated_scan_bwd(x, h, x, x, st[:0])),
-        (ValueError, lambda: gated_scan_step(x[0], x[0], h.t())),
+        (ValueError, lambda: gated_scan_fwd(x, x)),  # not on a GPU
+        (ValueError, lambda: gated_scan_bwd(x, h, x, x, st)),
+        (ValueError, lambda: ext().gated_scan_step(x[0], x[0], h.t(), None)),
+        (ValueError, lambda: ext().gated_scan_step(x[0], x[0], h, None)),
+        (ValueError, lambda: ext().gated_scan_step(
+            x[0], x[0], h.clone().requires_grad_(True), None)),
         (ValueError, lambda: gated_scan_step(
             x[0], x[0], torch.zeros(2, 12)[:, ::2])),
     ]
@@ -677,24 +688,25 @@ def test_logp_edges(device):
 def test_logp_refusals():
     x, a = torch.zeros(4, 8), torch.zeros(4, dtype=torch.int64)
     cases = [
-        (ValueError, lambda: action_logprobs(torch.zeros(()), a)),
-        (ValueError, lambda: action_logprobs(torch.zeros(4, 0), a)),
-        (TypeError, lambda: action_logprobs(x.double(), a)),
-        (ValueError, lambda: action_logprobs(x, a[:3])),
-        (ValueError, lambda: action_logprobs(x, a.int())),
-        (ValueError, lambda: action_logprobs(x, a, torch.ones(4, 7).bool())),
-        (ValueError, lambda: action_logprobs(x, a, torch.ones(8).bool())),
-        (ValueError, lambda: action_logprobs(x, a, torch.ones(4, 8))),
-        (ValueError, lambda: action_logprobs(x, a, top_k=9)),
-        (ValueError, lambda: action_logprobs(x, a, top_k=-1)),
-        (ValueError, lambda: action_logprobs(
+        (ValueError, lambda: action_logprobs_fwd(torch.zeros(()), a)),
+        (ValueError, lambda: action_logprobs_fwd(torch.zeros(4, 0), a)),
+        (TypeError, lambda: action_logprobs_fwd(x.double(), a)),
+        (ValueError, lambda: action_logprobs_fwd(x, a[:3])),
+        (ValueError, lambda: action_logprobs_fwd(x, a.int())),
+        (ValueError, lambda: action_logprobs_fwd(x, a, torch.ones(4, 7).bool())),
+        (ValueError, lambda: action_logprobs_fwd(x, a, torch.ones(8).bool())),
+        (ValueError, lambda: action_logprobs_fwd(x, a, torch.ones(4, 8))),
+        (ValueError, lambda: action_logprobs_fwd(x, a, top_k=9)),
+        (ValueError, lambda: action_logprobs_fwd(x, a, top_k=-1)),
+        (ValueError, lambda: action_logprobs_fwd(
             torch.zeros(4, 100), a, top_k=65)),
-        (ValueError, lambda: action_logprobs(x, a.to("meta"))),
+        (ValueError, lambda: action_logprobs_fwd(x, a.to("meta"))),
         (ValueError, lambda: action_logprobs_bwd(
-            a.float()[:2], None, x, a, None, x[:, :2].contiguous(),
-            a.float())),
+            a.float()[:2], None, x, a, None, x[:, :3].contiguous())),
         (ValueError, lambda: action_logprobs_bwd(
-            a.float(), None, x, a, None, x[:3, :2].contiguous(), a.float())),
+            a.float(), None, x, a, None, x[:3, :3].contiguous())),
+        (ValueError, lambda: action_logprobs_fwd(x, a)),  # not on a GPU
+        (ValueError, lambda: action_logprobs(x, a, top_k=9)),
     ]
     for err, call in cases:
         with pytest.raises(err):
@@ -816,7 +828,7 @@ def all_calls(seed, small=True):
         lp, H_, st2, tl, ti = action_logprobs_fwd(t["logits"], t["act"],
                                                   t["mask"], 7)
         dl = action_logprobs_bwd(t["d"], lp.nan_to_num(0.0, 0.0, 0.0),
-                                 t["logits"], t["act"], t["mask"], st2, H_)
+                                 t["logits"], t["act"], t["mask"], st2)
         return [y, dx, dw, db, hs, hl, dg, dv, dh0, h, o, lp, H_, tl, ti, dl]
 
     return t, run
@@ -884,6 +896,10 @@ def test_captured_autograd_and_its_refusal():
         with torch.cuda.graph(torch.cuda.CUDAGraph()):
             layer_norm(x, w)
     want, = torch.autograd.grad(eager.square().sum(), w)
+    # nor where other operators lie between the leaf and the call
+    with pytest.raises(RuntimeError, match="alive"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            gated_scan(x.expand(2, 5, 16), (x * w).expand(2, 5, 16))
     del eager
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
@@ -898,6 +914,16 @@ def test_captured_autograd_and_its_refusal():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
+def test_second_derivatives_are_refused():
+    x = torch.randn(4, 3, 8, device="cuda", requires_grad=True)
+    act = torch.zeros(4, 3, dtype=torch.int64, device="cuda")
+    for y in (layer_norm(x), gated_scan(x, x)[0],
+              action_logprobs(x, act).logp):
+        with pytest.raises(RuntimeError, match="create_graph"):
+            torch.autograd.grad(y.sum(), x, create_graph=True)
 
 
 @pytest.mark.gpu
@@ -918,7 +944,7 @@ def test_offsets_past_32_bits():
     act = torch.randint(0, A, (32800,), device=dev)
     lp, H, st2, tl, ti = action_logprobs_fwd(z, act, None, 4)
     d = torch.ones_like(lp)
-    dz = action_logprobs_bwd(d, d, z, act, None, st2, H)
+    dz = action_logprobs_bwd(d, d, z, act, None, st2)
     want = logp_64(z[-2:], act[-2:], None, 4, d[-2:], d[-2:])
     close(lp[-2:], *want["logp"], "logp")
     close(H[-2:], *want["entropy"], "entropy")
