@@ -41,7 +41,8 @@ def __getattr__(name):
     if name in _EXPORTS:
         import importlib
         mod = importlib.import_module(_EXPORTS[name])
-        return getattr(mod, name)
+        globals()[name] = getattr(mod, name)   # found at once from now on
+        return globals()[name]
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
 
 

@@ -16,15 +16,24 @@ enum Type { F32 = 0, BF16 = 1, F16 = 2 };
 typedef __bf16 bf16;
 typedef _Float16 f16;
 
-// N elements as one load or store of N * sizeof(T) bytes (at most 16)
+// N elements as one load or store of N * sizeof(T) bytes, at any address:
+// global accesses of this part need no alignment beyond the byte's, so rows
+// of odd lengths go the same way as even ones.
 template <typename T, int N>
-struct alignas(sizeof(T) * N) Vec {
+struct Vec {
   T v[N];
 };
 
 template <typename T, int N>
+__device__ __forceinline__ Vec<T, N> load(const T* p) {
+  Vec<T, N> r;
+  __builtin_memcpy(&r, p, sizeof(r));
+  return r;
+}
+
+template <typename T, int N>
 __device__ __forceinline__ void load(const T* p, float (&f)[N]) {
-  Vec<T, N> r = *reinterpret_cast<const Vec<T, N>*>(p);
+  const Vec<T, N> r = load<T, N>(p);
 #pragma unroll
   for (int i = 0; i < N; ++i) f[i] = (float)r.v[i];
 }
@@ -35,13 +44,25 @@ __device__ __forceinline__ void store(T* p, const float (&f)[N]) {
   Vec<T, N> r;
 #pragma unroll
   for (int i = 0; i < N; ++i) r.v[i] = (T)f[i];
-  *reinterpret_cast<Vec<T, N>*>(p) = r;
+  __builtin_memcpy(p, &r, sizeof(r));
+}
+
+// Of two values the larger, and NaN if either is (one instruction).
+__device__ __forceinline__ float maximum(float a, float b) {
+  return __builtin_elementwise_maximum(a, b);
 }
 
 template <int W = kWave>
 __device__ __forceinline__ float group_sum(float v) {
 #pragma unroll
   for (int o = W / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, kWave);
+  return v;
+}
+
+template <int W = kWave>
+__device__ __forceinline__ float group_max(float v) {
+#pragma unroll
+  for (int o = W / 2; o > 0; o >>= 1) v = maximum(v, __shfl_xor(v, o, kWave));
   return v;
 }
 
@@ -69,10 +90,6 @@ inline hipError_t launch(void (*kernel)(P...), dim3 grid, dim3 block,
   void* list[] = {(void*)&args...};
   static_assert(sizeof...(P) == sizeof...(A), "one value for each parameter");
   return hipLaunchKernel((const void*)kernel, grid, block, list, lds, stream);
-}
-
-inline bool aligned(const void* p, int64_t bytes) {
-  return ((uintptr_t)p & (uintptr_t)(bytes - 1)) == 0;
 }
 
 }  // namespace seq
