@@ -9,14 +9,56 @@
 // A reset is a selection, not a product: nothing before an episode's end,
 // not even a NaN, is seen after it. The state is held in 32 bits throughout;
 // the backward pass does not read the rounded hs but computes c again from
-// the 32-bit states kept at every kKeep-th step.
+// the 32-bit states kept at every kKeep-th step, which also reads less.
+//
+// A lane owns V neighbouring columns of one environment and walks time. With
+// columns enough for the chip it walks all of it, in one pass. With fewer,
+// time is cut into chunks: a first kernel finds each chunk's effect on the
+// state, c_end = A c_start + B, a second joins those from chunk to chunk,
+// and a third walks every chunk from its own start.
 #include "seq_api.h"
 #include "seq_common.h"
 
 namespace {
 using namespace seq;
 
-constexpr int kKeep = 64;  // steps from one kept state to the next
+constexpr int kKeep = 16;  // steps from one kept state to the next
+
+// A sequence's columns as lanes: n lanes an environment, the last of which
+// begins early enough to end with it and computes shared columns twice, to
+// the same bits.
+struct Cols {
+  int64_t E, H, n;
+};
+
+// A lane's environment and columns, counted from the block's first
+// environment e0: what is far is the same for the block, and a lane's own
+// distance fits 32 bits (the host sees to it).
+struct Lane {
+  int64_t e0;
+  uint32_t e, i;
+};
+
+template <int V>
+__device__ __forceinline__ bool lane_of(const Cols& c, Lane& l) {
+  const int64_t g0 = (int64_t)blockIdx.x * 256;
+  l.e0 = g0 / c.n;
+  const uint32_t n = (uint32_t)c.n, H = (uint32_t)c.H;
+  const uint32_t r = (uint32_t)(g0 - l.e0 * c.n) + threadIdx.x;
+  l.e = r / n;
+  if (l.e0 + l.e >= c.E) return false;
+  const uint32_t i = (r - l.e * n) * V;
+  l.i = i < H - V ? i : H - V;
+  return true;
+}
+
+// One step's values of a lane's environment and columns: `at` is the step's,
+// stride_e from one environment to the next.
+template <typename T>
+__device__ __forceinline__ T* here(T* at, const Lane& l, int64_t stride_e) {
+  const uint32_t own = (l.e * (uint32_t)stride_e + l.i) * sizeof(T);
+  return (T*)((char*)(at + l.e0 * stride_e) + own);
+}
 
 struct ScanFwd {
   const void* gate;
@@ -26,7 +68,9 @@ struct ScanFwd {
   void* hs;
   float* h_last;
   float* states;  // [ceil(T / kKeep), E, H]: c at t = 0, kKeep, ...; or null
-  int64_t T, E, H;
+  float* carry;   // [chunks, E, H]: c at the chunks' starts; null: one chunk
+  Cols c;
+  int64_t T, chunk;
   int64_t gate_t, gate_e, x_t, x_e;  // strides of time and environment
 };
 
@@ -39,132 +83,540 @@ struct ScanBwd {
   const uint8_t* done;
   void* dgate;
   void* dx;
-  float* dh0;  // null: not asked for
-  int64_t T, E, H;
+  float* dh0;    // null: not asked for
+  float* carry;  // [chunks, E, H]: a D of the step behind each chunk
+  Cols c;
+  int64_t T, chunk;
   int64_t gate_t, gate_e, x_t, x_e, dhs_t, dhs_e;
 };
 
 // z and 1 - z, each to its own last bits: neither is taken as a difference.
 __device__ __forceinline__ void gates(float g, float& z, float& a) {
   const float e = __expf(-fabsf(g));
-  const float r = __frcp_rn(1.f + e);
+  const float r = __builtin_amdgcn_rcpf(1.f + e);
   const float q = e * r;
   z = g >= 0.f ? r : q;
   a = g >= 0.f ? q : r;
   if (g != g) z = a = g;
 }
 
-template <typename T>
+// A state's way through some steps: c_end = A c_start + B, or B alone (A
+// below zero) where an episode ended within them.
+struct Way {
+  float A = 1.f, B = 0.f;
+  __device__ __forceinline__ void step(float a, float b) {
+    A = A < 0.f ? A : A * a;
+    B = a * B + b;
+  }
+  __device__ __forceinline__ void end() {
+    A = -1.f;
+    B = 0.f;
+  }
+  __device__ __forceinline__ void then(float a, float b) {
+    B = a < 0.f ? b : a * B + b;
+    A = a < 0.f || A < 0.f ? -1.f : A * a;
+  }
+};
+
+// ---- forward
+// The k-th step from t, or the last before `end`: what is behind it is read
+// there and not used. FULL: there is nothing behind it.
+template <bool FULL>
+__device__ __forceinline__ int64_t step_at(int64_t t, int k, int64_t end) {
+  return FULL || t + k < end ? k : end - 1 - t;
+}
+
+// L steps of a lane's columns, and which of them end an episode.
+template <typename T, int V, int L>
+struct Steps {
+  Vec<T, V> gate[L], x[L];
+  uint32_t ends;
+
+  template <bool FULL>
+  __device__ __forceinline__ void read(const ScanFwd& p, const Lane& l,
+                                       int64_t t, int64_t end) {
+    const T* g = here((const T*)p.gate + t * p.gate_t, l, p.gate_e);
+    const T* v = here((const T*)p.x + t * p.x_t, l, p.x_e);
+#pragma unroll
+    for (int k = 0; k < L; ++k) {
+      const int64_t i = step_at<FULL>(t, k, end);
+      gate[k] = load<T, V>(g + i * p.gate_t);
+      x[k] = load<T, V>(v + i * p.x_t);
+    }
+    ends = 0;
+    if (p.done) {
+      const uint8_t* d = p.done + t * p.c.E + l.e0 + l.e;
+#pragma unroll
+      for (int k = 0; k < L; ++k)
+        ends |= (uint32_t)(d[step_at<FULL>(t, k, end) * p.c.E] != 0) << k;
+    }
+  }
+};
+
+template <bool FULL, typename T, int V, int L>
+__device__ __forceinline__ void walk(const ScanFwd& p, const Lane& l,
+                                     const Steps<T, V, L>& s, int64_t t,
+                                     int64_t end, float (&c)[V]) {
+  const int64_t EH = p.c.E * p.c.H;
+  if (p.states && t % kKeep == 0)
+    store<float, V>(here(p.states + t / kKeep * EH, l, p.c.H), c);
+  T* out = here((T*)p.hs + t * EH, l, p.c.H);
+#pragma unroll
+  for (int k = 0; k < L; ++k) {
+    if (!FULL && t + k >= end) continue;
+    float h[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      float z, a;
+      gates((float)s.gate[k].v[v], z, a);
+      h[v] = a * c[v] + z * (float)s.x[k].v[v];
+      c[v] = s.ends >> k & 1 ? 0.f : h[v];
+    }
+    store<T, V>(out + k * EH, h);
+  }
+}
+
+// kKeep is a multiple of L and a chunk one of kKeep, so states lie at the
+// first of L steps.
+template <typename T, int V, int L>
 __global__ __launch_bounds__(256) void scan_fwd_kernel(ScanFwd p) {
-  const int64_t col = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (col >= p.E * p.H) return;
-  const int64_t e = col / p.H, i = col % p.H;
-  float c = p.h0 ? p.h0[col] : 0.f;
-  for (int64_t t = 0; t < p.T; ++t) {
-    if (p.states && t % kKeep == 0) p.states[t / kKeep * p.E * p.H + col] = c;
-    float z, a;
-    gates((float)((const T*)p.gate)[t * p.gate_t + e * p.gate_e + i], z, a);
-    const float x = (float)((const T*)p.x)[t * p.x_t + e * p.x_e + i];
-    const float h = a * c + z * x;
-    ((T*)p.hs)[t * p.E * p.H + col] = (T)h;
-    c = p.done && p.done[t * p.E + e] ? 0.f : h;
+  static_assert(kKeep % L == 0, "states are kept between steps read at once");
+  Lane l;
+  if (!lane_of<V>(p.c, l)) return;
+  const int64_t EH = p.c.E * p.c.H;
+  int64_t t = blockIdx.y * p.chunk;
+  const int64_t end = t + p.chunk < p.T ? t + p.chunk : p.T;
+  float c[V] = {};
+  if (p.carry) {
+    load<float, V>(here(p.carry + blockIdx.y * EH, l, p.c.H), c);
+  } else if (p.h0) {
+    load<float, V>(here(p.h0, l, p.c.H), c);
   }
-  p.h_last[col] = c;
+  if (t + L <= end) {
+    // the next steps are read while these are walked
+    Steps<T, V, L> s, n;
+    s.template read<true>(p, l, t, end);
+    for (; t + 2 * L <= end; t += L) {
+      n.template read<true>(p, l, t + L, end);
+      walk<true>(p, l, s, t, end, c);
+      s = n;
+    }
+    walk<true>(p, l, s, t, end, c);
+    t += L;
+  }
+  if (t < end) {
+    Steps<T, V, L> s;
+    s.template read<false>(p, l, t, end);
+    walk<false>(p, l, s, t, end, c);
+  }
+  if (end == p.T) store<float, V>(here(p.h_last, l, p.c.H), c);
 }
 
-template <typename T>
+template <bool FULL, typename T, int V, int L>
+__device__ __forceinline__ void way(const ScanFwd& p, const Lane& l, int64_t t,
+                                    int64_t end, Way (&w)[V]) {
+  Steps<T, V, L> s;
+  s.template read<FULL>(p, l, t, end);
+#pragma unroll
+  for (int k = 0; k < L; ++k) {
+    if (!FULL && t + k >= end) continue;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      float z, a;
+      gates((float)s.gate[k].v[v], z, a);
+      w[v].step(a, z * (float)s.x[k].v[v]);
+      if (s.ends >> k & 1) w[v].end();
+    }
+  }
+}
+
+template <int V>
+__device__ __forceinline__ void keep_way(const Cols& c, const Lane& l,
+                                         const Way (&w)[V], float* ways) {
+  float A[V], B[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) A[v] = w[v].A, B[v] = w[v].B;
+  const int64_t EH = c.E * c.H, k = blockIdx.y;
+  store<float, V>(here(ways + 2 * k * EH, l, c.H), A);
+  store<float, V>(here(ways + (2 * k + 1) * EH, l, c.H), B);
+}
+
+template <typename T, int V>
+__global__ __launch_bounds__(256) void scan_fwd_way_kernel(ScanFwd p,
+                                                           float* ways) {
+  constexpr int L = kKeep;
+  Lane l;
+  if (!lane_of<V>(p.c, l)) return;
+  int64_t t = blockIdx.y * p.chunk;
+  const int64_t end = t + p.chunk < p.T ? t + p.chunk : p.T;
+  Way w[V];
+  for (; t + L <= end; t += L) way<true, T, V, L>(p, l, t, end, w);
+  if (t < end) way<false, T, V, L>(p, l, t, end, w);
+  keep_way<V>(p.c, l, w, ways);
+}
+
+// ---- from chunk to chunk, in either direction: 64 columns a block, its 16
+// waves one after the other in time, kJoin chunks each
+constexpr int kJoin = 8;
+
+struct Join {
+  const float* ways;   // [chunks, 2, EH]
+  const float* first;  // [EH] or null: zeros
+  float* carry;        // [chunks, EH]
+  int64_t EH, chunks;
+  bool reverse;
+};
+
+__global__ __launch_bounds__(1024) void scan_join_kernel(Join p) {
+  __shared__ float lds[2][16][2][kWave];
+  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+  const int64_t col = (int64_t)blockIdx.x * kWave + lane;
+  const bool mine = col < p.EH;
+  float c = mine && p.first ? p.first[col] : 0.f;
+  int turn = 0;
+  for (int64_t k0 = 0; k0 < p.chunks; k0 += 16 * kJoin, turn ^= 1) {
+    const int64_t k = k0 + wave * kJoin;
+    float A[kJoin], B[kJoin];
+    Way w;
+#pragma unroll
+    for (int i = 0; i < kJoin; ++i) {
+      A[i] = 1.f;
+      B[i] = 0.f;
+      if (k + i < p.chunks && mine) {
+        const int64_t at = p.reverse ? p.chunks - 1 - (k + i) : k + i;
+        A[i] = p.ways[2 * at * p.EH + col];
+        B[i] = p.ways[(2 * at + 1) * p.EH + col];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kJoin; ++i) w.then(A[i], B[i]);
+    lds[turn][wave][0][lane] = w.A;
+    lds[turn][wave][1][lane] = w.B;
+    // one barrier a turn: the next turn writes the other half
+    __syncthreads();
+    float start = c;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      if (i == wave) start = c;
+      const float a = lds[turn][i][0][lane], b = lds[turn][i][1][lane];
+      c = a < 0.f ? b : a * c + b;
+    }
+#pragma unroll
+    for (int i = 0; i < kJoin; ++i) {
+      if (k + i < p.chunks && mine) {
+        const int64_t at = p.reverse ? p.chunks - 1 - (k + i) : k + i;
+        p.carry[at * p.EH + col] = start;
+      }
+      start = A[i] < 0.f ? B[i] : A[i] * start + B[i];
+    }
+  }
+}
+
+// ---- backward
+// kKeep steps of a lane's columns.
+template <typename T, int V>
+struct Back {
+  Vec<T, V> gate[kKeep], dhs[kKeep];
+  uint32_t ends = 0;
+
+  template <bool FULL>
+  __device__ __forceinline__ void read(const ScanBwd& p, const Lane& l,
+                                       int64_t t, int64_t end) {
+    const T* g = here((const T*)p.gate + t * p.gate_t, l, p.gate_e);
+#pragma unroll
+    for (int k = 0; k < kKeep; ++k)
+      gate[k] = load<T, V>(g + step_at<FULL>(t, k, end) * p.gate_t);
+    if (p.dhs) {
+      const T* h = here((const T*)p.dhs + t * p.dhs_t, l, p.dhs_e);
+#pragma unroll
+      for (int k = 0; k < kKeep; ++k)
+        dhs[k] = load<T, V>(h + step_at<FULL>(t, k, end) * p.dhs_t);
+    } else {
+#pragma unroll
+      for (int k = 0; k < kKeep; ++k) dhs[k] = {};
+    }
+    if (p.done) {
+      const uint8_t* d = p.done + t * p.c.E + l.e0 + l.e;
+#pragma unroll
+      for (int k = 0; k < kKeep; ++k)
+        ends |= (uint32_t)(d[step_at<FULL>(t, k, end) * p.c.E] != 0) << k;
+    }
+  }
+};
+
+template <bool FULL, typename T, int V>
+__device__ __forceinline__ void way_back(const ScanBwd& p, const Lane& l,
+                                         int64_t t, int64_t end, Way (&w)[V]) {
+  Back<T, V> s;
+  s.template read<FULL>(p, l, t, end);
+#pragma unroll
+  for (int k = kKeep - 1; k >= 0; --k) {
+    if (!FULL && t + k >= end) continue;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      float z, a;
+      gates((float)s.gate[k].v[v], z, a);
+      if (s.ends >> k & 1) w[v].end();
+      w[v].step(a, a * (float)s.dhs[k].v[v]);
+    }
+  }
+}
+
+template <typename T, int V>
+__global__ __launch_bounds__(256) void scan_bwd_way_kernel(ScanBwd p,
+                                                           float* ways) {
+  Lane l;
+  if (!lane_of<V>(p.c, l)) return;
+  const int64_t t0 = blockIdx.y * p.chunk;
+  const int64_t end = t0 + p.chunk < p.T ? t0 + p.chunk : p.T;
+  int64_t t = t0 + (end - t0) / kKeep * kKeep;
+  Way w[V];
+  if (t < end) way_back<false, T, V>(p, l, t, end, w);
+  for (t -= kKeep; t >= t0; t -= kKeep)
+    way_back<true, T, V>(p, l, t, end, w);
+  keep_way<V>(p.c, l, w, ways);
+}
+
+template <bool FULL, typename T, int V>
+__device__ __forceinline__ void walk_back(const ScanBwd& p, const Lane& l,
+                                          int64_t t, int64_t end,
+                                          float (&carry)[V]) {
+  const int64_t EH = p.c.E * p.c.H;
+  Back<T, V> s;
+  Vec<T, V> x[kKeep];
+  float c[V], diff[kKeep][V];  // x - c
+  load<float, V>(here(p.states + t / kKeep * EH, l, p.c.H), c);
+  const T* v0 = here((const T*)p.x + t * p.x_t, l, p.x_e);
+#pragma unroll
+  for (int k = 0; k < kKeep; ++k)
+    x[k] = load<T, V>(v0 + step_at<FULL>(t, k, end) * p.x_t);
+  s.template read<FULL>(p, l, t, end);
+#pragma unroll
+  for (int k = 0; k < kKeep; ++k) {
+    if (!FULL && t + k >= end) continue;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      float z, a;
+      gates((float)s.gate[k].v[v], z, a);
+      const float xv = (float)x[k].v[v];
+      diff[k][v] = xv - c[v];
+      c[v] = s.ends >> k & 1 ? 0.f : a * c[v] + z * xv;
+    }
+  }
+  T* out_x = here((T*)p.dx + t * EH, l, p.c.H);
+  T* out_g = here((T*)p.dgate + t * EH, l, p.c.H);
+#pragma unroll
+  for (int k = kKeep - 1; k >= 0; --k) {
+    if (!FULL && t + k >= end) continue;
+    float dg[V], dx[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      float z, a;
+      gates((float)s.gate[k].v[v], z, a);
+      const float D =
+          (s.ends >> k & 1 ? 0.f : carry[v]) + (float)s.dhs[k].v[v];
+      dx[v] = z * D;
+      dg[v] = D * diff[k][v] * (z * a);
+      carry[v] = a * D;
+    }
+    store<T, V>(out_x + k * EH, dx);
+    store<T, V>(out_g + k * EH, dg);
+  }
+}
+
+template <typename T, int V>
 __global__ __launch_bounds__(256) void scan_bwd_kernel(ScanBwd p) {
-  const int64_t col = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (col >= p.E * p.H) return;
-  const int64_t e = col / p.H, i = col % p.H;
-  float carry = p.dh_last ? p.dh_last[col] : 0.f;  // a_{t+1} D_{t+1}
-  float before[kKeep];
-  for (int64_t t0 = (p.T - 1) / kKeep * kKeep; t0 >= 0; t0 -= kKeep) {
-    const int n = (int)(p.T - t0 < kKeep ? p.T - t0 : kKeep);
-    float c = p.states[t0 / kKeep * p.E * p.H + col];
-    for (int k = 0; k < n; ++k) {
-      const int64_t t = t0 + k;
-      before[k] = c;
-      float z, a;
-      gates((float)((const T*)p.gate)[t * p.gate_t + e * p.gate_e + i], z, a);
-      const float x = (float)((const T*)p.x)[t * p.x_t + e * p.x_e + i];
-      const float h = a * c + z * x;
-      c = p.done && p.done[t * p.E + e] ? 0.f : h;
-    }
-    for (int k = n - 1; k >= 0; --k) {
-      const int64_t t = t0 + k;
-      float z, a;
-      gates((float)((const T*)p.gate)[t * p.gate_t + e * p.gate_e + i], z, a);
-      const float x = (float)((const T*)p.x)[t * p.x_t + e * p.x_e + i];
-      float d = p.done && p.done[t * p.E + e] ? 0.f : carry;
-      if (p.dhs) d += (float)((const T*)p.dhs)[t * p.dhs_t + e * p.dhs_e + i];
-      ((T*)p.dx)[t * p.E * p.H + col] = (T)(z * d);
-      ((T*)p.dgate)[t * p.E * p.H + col] = (T)(d * (x - before[k]) * z * a);
-      carry = a * d;
-    }
+  Lane l;
+  if (!lane_of<V>(p.c, l)) return;
+  const int64_t EH = p.c.E * p.c.H;
+  const int64_t t0 = blockIdx.y * p.chunk;
+  const int64_t end = t0 + p.chunk < p.T ? t0 + p.chunk : p.T;
+  float carry[V] = {};  // a_{t+1} D_{t+1}
+  if (p.carry) {
+    load<float, V>(here(p.carry + blockIdx.y * EH, l, p.c.H), carry);
+  } else if (p.dh_last) {
+    load<float, V>(here(p.dh_last, l, p.c.H), carry);
   }
-  if (p.dh0) p.dh0[col] = carry;
+  int64_t t = t0 + (end - t0) / kKeep * kKeep;
+  if (t < end) walk_back<false, T, V>(p, l, t, end, carry);
+  for (t -= kKeep; t >= t0; t -= kKeep)
+    walk_back<true, T, V>(p, l, t, end, carry);
+  if (t0 == 0 && p.dh0) store<float, V>(here(p.dh0, l, p.c.H), carry);
 }
 
+// ---- one step
 struct ScanStep {
   const void* gate;
   const void* x;
   const uint8_t* done;  // environments that restart from zero; null: none
   float* h;             // in place
   void* hs;
-  int64_t E, H, gate_e, x_e;
+  Cols c;
+  int64_t gate_e, x_e;
 };
 
-template <typename T>
+template <typename T, int V>
 __global__ __launch_bounds__(256) void scan_step_kernel(ScanStep p) {
-  const int64_t col = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (col >= p.E * p.H) return;
-  const int64_t e = col / p.H, i = col % p.H;
-  const float c = p.done && p.done[e] ? 0.f : p.h[col];
-  float z, a;
-  gates((float)((const T*)p.gate)[e * p.gate_e + i], z, a);
-  const float h = a * c + z * (float)((const T*)p.x)[e * p.x_e + i];
-  p.h[col] = h;
-  ((T*)p.hs)[col] = (T)h;
+  Lane l;
+  if (!lane_of<V>(p.c, l)) return;
+  const bool end = p.done && p.done[l.e0 + l.e];
+  const Vec<T, V> gate = load<T, V>(here((const T*)p.gate, l, p.gate_e));
+  const Vec<T, V> x = load<T, V>(here((const T*)p.x, l, p.x_e));
+  float h[V];
+  load<float, V>(here(p.h, l, p.c.H), h);
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    float z, a;
+    gates((float)gate.v[v], z, a);
+    h[v] = a * (end ? 0.f : h[v]) + z * (float)x.v[v];
+  }
+  store<float, V>(here(p.h, l, p.c.H), h);
+  store<T, V>(here((T*)p.hs, l, p.c.H), h);
+}
+
+// In place, so no column may be computed twice: V divides H.
+template <typename T, int V>
+hipError_t step_with(ScanStep p, hipStream_t s) {
+  p.c.n = p.c.H / V;
+  const int64_t grid = (p.c.E * p.c.n + 255) / 256;
+  return launch(scan_step_kernel<T, V>, dim3(grid), dim3(256), 0, s, p);
 }
 
 template <typename T>
 hipError_t step(const ScanStep& p, hipStream_t s) {
-  if (p.E * p.H == 0) return hipSuccess;
-  const int64_t grid = (p.E * p.H + 255) / 256;
-  return launch(scan_step_kernel<T>, dim3(grid), dim3(256), 0, s, p);
+  if (p.c.E * p.c.H == 0) return hipSuccess;
+  if (p.c.H % 4 == 0) return step_with<T, 4>(p, s);
+  if (p.c.H % 2 == 0) return step_with<T, 2>(p, s);
+  return step_with<T, 1>(p, s);
+}
+
+// How the columns of a call lie on lanes, and its time in chunks.
+struct Plan {
+  int V;
+  int64_t n, chunk, chunks;
+};
+
+constexpr int64_t kWaves = 2048;  // as many keep the memory busy
+constexpr int64_t kShort = 128;   // steps that one lane walks in any case
+
+Plan plan(int64_t T, int64_t E, int64_t H) {
+  Plan p;
+  p.V = H < 2 ? 1 : 2;
+  p.n = (H + p.V - 1) / p.V;
+  const int64_t waves = (E * p.n + kWave - 1) / kWave;
+  p.chunk = T;
+  p.chunks = 1;
+  if (T > kShort && waves < kWaves) {
+    int64_t want = 2 * kWaves / waves;  // chunks
+    const int64_t most = (T + 63) / 64;
+    want = want < most ? want : most;
+    want = want < 32768 ? want : 32768;
+    if (want > 1) {
+      p.chunk = (T + want - 1) / want;
+      p.chunk = (p.chunk + kKeep - 1) / kKeep * kKeep;
+      p.chunks = (T + p.chunk - 1) / p.chunk;
+    }
+  }
+  return p;
+}
+
+// scratch: the chunks' ways and their carries
+float* carry_of(const Plan& q, float* scratch, int64_t EH) {
+  return q.chunks > 1 ? scratch + 2 * q.chunks * EH : nullptr;
+}
+
+hipError_t join(const float* ways, const float* first, float* carry,
+                const Plan& q, int64_t EH, bool reverse, hipStream_t s) {
+  const Join j = {ways, first, carry, EH, q.chunks, reverse};
+  return launch(scan_join_kernel, dim3((EH + kWave - 1) / kWave), dim3(1024),
+                0, s, j);
+}
+
+template <typename T, int V, int L>
+hipError_t fwd_with(const ScanFwd& p, const Plan& q, float* ways,
+                    hipStream_t s) {
+  const int64_t EH = p.c.E * p.c.H;
+  const dim3 grid((p.c.E * p.c.n + 255) / 256, q.chunks);
+  if (q.chunks > 1) {
+    hipError_t e = launch(scan_fwd_way_kernel<T, V>, grid, dim3(256), 0, s,
+                          p, ways);
+    if (e == hipSuccess) e = join(ways, p.h0, p.carry, q, EH, false, s);
+    if (e != hipSuccess) return e;
+  }
+  return launch(scan_fwd_kernel<T, V, L>, grid, dim3(256), 0, s, p);
 }
 
 template <typename T>
-hipError_t fwd(const ScanFwd& p, hipStream_t s) {
-  if (p.E * p.H == 0) return hipSuccess;
-  const int64_t grid = (p.E * p.H + 255) / 256;
-  return launch(scan_fwd_kernel<T>, dim3(grid), dim3(256), 0, s, p);
+hipError_t fwd(ScanFwd p, float* scratch, hipStream_t s) {
+  if (p.c.E * p.c.H == 0) return hipSuccess;
+  const Plan q = plan(p.T, p.c.E, p.c.H);
+  p.c.n = q.n;
+  p.chunk = q.chunk;
+  p.carry = carry_of(q, scratch, p.c.E * p.c.H);
+  if (q.V == 2) return fwd_with<T, 2, 8>(p, q, scratch, s);
+  return fwd_with<T, 1, 8>(p, q, scratch, s);
+}
+
+template <typename T, int V>
+hipError_t bwd_with(const ScanBwd& p, const Plan& q, float* ways,
+                    hipStream_t s) {
+  const int64_t EH = p.c.E * p.c.H;
+  const dim3 grid((p.c.E * p.c.n + 255) / 256, q.chunks);
+  if (q.chunks > 1) {
+    hipError_t e =
+        launch(scan_bwd_way_kernel<T, V>, grid, dim3(256), 0, s, p, ways);
+    if (e == hipSuccess) e = join(ways, p.dh_last, p.carry, q, EH, true, s);
+    if (e != hipSuccess) return e;
+  }
+  return launch(scan_bwd_kernel<T, V>, grid, dim3(256), 0, s, p);
 }
 
 template <typename T>
-hipError_t bwd(const ScanBwd& p, hipStream_t s) {
-  if (p.E * p.H == 0) return hipSuccess;
-  const int64_t grid = (p.E * p.H + 255) / 256;
-  return launch(scan_bwd_kernel<T>, dim3(grid), dim3(256), 0, s, p);
+hipError_t bwd(ScanBwd p, float* scratch, hipStream_t s) {
+  if (p.c.E * p.c.H == 0) return hipSuccess;
+  const Plan q = plan(p.T, p.c.E, p.c.H);
+  p.c.n = q.n;
+  p.chunk = q.chunk;
+  p.carry = carry_of(q, scratch, p.c.E * p.c.H);
+  if (q.V == 2) return bwd_with<T, 2>(p, q, scratch, s);
+  return bwd_with<T, 1>(p, q, scratch, s);
 }
 
 }  // namespace
 
+// Floats of scratch that the forward and the backward call each need.
+extern "C" int64_t rlsched_scan_scratch(int64_t T, int64_t E, int64_t H) {
+  if (E * H == 0) return 0;
+  const Plan q = plan(T, E, H);
+  return q.chunks > 1 ? 3 * q.chunks * E * H : 0;
+}
+
+// Elements from one environment to the next that a lane's 32-bit distance
+// covers for any number of them in a block; beyond it the caller copies.
+extern "C" int64_t rlsched_scan_reach(int64_t H) {
+  const int64_t envs = 256 * 4 / (H < 1 ? 1 : H) + 2;
+  return ((1ll << 31) / 4 - H) / (envs < 256 ? envs : 256);
+}
+
+extern "C" int64_t rlsched_scan_states(int64_t T) {
+  return (T + kKeep - 1) / kKeep;
+}
+
 extern "C" int rlsched_scan_fwd(int device, void* stream, const void* gate,
                                 const void* x, const float* h0,
                                 const uint8_t* done, void* hs, float* h_last,
-                                float* states, int64_t T, int64_t E, int64_t H,
-                                int64_t gate_t, int64_t gate_e, int64_t x_t,
-                                int64_t x_e, int type) {
+                                float* states, float* scratch, int64_t T,
+                                int64_t E, int64_t H, int64_t gate_t,
+                                int64_t gate_e, int64_t x_t, int64_t x_e,
+                                int type) {
   OnDevice on(device);
   if (on.err != hipSuccess) return on.err;
-  const ScanFwd p = {gate, x, h0, done,   hs,     h_last, states, T,
-                     E,    H, gate_t, gate_e, x_t,    x_e};
+  const ScanFwd p = {gate,   x, h0, done, hs, h_last, states, nullptr,
+                     {E, H}, T, 0,  gate_t, gate_e, x_t, x_e};
   const hipStream_t s = (hipStream_t)stream;
-  if (type == F32) return fwd<float>(p, s);
-  if (type == BF16) return fwd<bf16>(p, s);
-  if (type == F16) return fwd<f16>(p, s);
+  if (type == F32) return fwd<float>(p, scratch, s);
+  if (type == BF16) return fwd<bf16>(p, scratch, s);
+  if (type == F16) return fwd<f16>(p, scratch, s);
   return hipErrorInvalidValue;
 }
 
@@ -172,19 +624,19 @@ extern "C" int rlsched_scan_bwd(int device, void* stream, const void* dhs,
                                 const float* dh_last, const void* gate,
                                 const void* x, const float* states,
                                 const uint8_t* done, void* dgate, void* dx,
-                                float* dh0, int64_t T, int64_t E, int64_t H,
-                                int64_t gate_t, int64_t gate_e, int64_t x_t,
-                                int64_t x_e, int64_t dhs_t, int64_t dhs_e,
-                                int type) {
+                                float* dh0, float* scratch, int64_t T,
+                                int64_t E, int64_t H, int64_t gate_t,
+                                int64_t gate_e, int64_t x_t, int64_t x_e,
+                                int64_t dhs_t, int64_t dhs_e, int type) {
   OnDevice on(device);
   if (on.err != hipSuccess) return on.err;
-  const ScanBwd p = {dhs, dh_last, gate,   x,      states, done,  dgate,
-                     dx,  dh0,     T,      E,      H,      gate_t, gate_e,
-                     x_t, x_e,     dhs_t,  dhs_e};
+  const ScanBwd p = {dhs, dh_last, gate,    x,      states, done, dgate,
+                     dx,  dh0,     nullptr, {E, H}, T,      0,    gate_t,
+                     gate_e, x_t,  x_e,     dhs_t,  dhs_e};
   const hipStream_t s = (hipStream_t)stream;
-  if (type == F32) return bwd<float>(p, s);
-  if (type == BF16) return bwd<bf16>(p, s);
-  if (type == F16) return bwd<f16>(p, s);
+  if (type == F32) return bwd<float>(p, scratch, s);
+  if (type == BF16) return bwd<bf16>(p, scratch, s);
+  if (type == F16) return bwd<f16>(p, scratch, s);
   return hipErrorInvalidValue;
 }
 
@@ -194,7 +646,7 @@ extern "C" int rlsched_scan_step(int device, void* stream, const void* gate,
                                  int64_t gate_e, int64_t x_e, int type) {
   OnDevice on(device);
   if (on.err != hipSuccess) return on.err;
-  const ScanStep p = {gate, x, done, h, hs, E, H, gate_e, x_e};
+  const ScanStep p = {gate, x, done, h, hs, {E, H}, gate_e, x_e};
   const hipStream_t s = (hipStream_t)stream;
   if (type == F32) return step<float>(p, s);
   if (type == BF16) return step<bf16>(p, s);

@@ -17,17 +17,21 @@ int rlsched_norm_bwd(int device, void* stream, const void* dy, const void* x,
                      int64_t rows, int64_t dim, int64_t x_stride,
                      int64_t dy_stride, int type, int wtype);
 
+int64_t rlsched_scan_scratch(int64_t T, int64_t E, int64_t H);
+int64_t rlsched_scan_states(int64_t T);
+int64_t rlsched_scan_reach(int64_t H);
 int rlsched_scan_fwd(int device, void* stream, const void* gate, const void* x,
                      const float* h0, const uint8_t* done, void* hs,
-                     float* h_last, float* states, int64_t T, int64_t E,
-                     int64_t H, int64_t gate_t, int64_t gate_e, int64_t x_t,
-                     int64_t x_e, int type);
+                     float* h_last, float* states, float* scratch, int64_t T,
+                     int64_t E, int64_t H, int64_t gate_t, int64_t gate_e,
+                     int64_t x_t, int64_t x_e, int type);
 int rlsched_scan_bwd(int device, void* stream, const void* dhs,
                      const float* dh_last, const void* gate, const void* x,
                      const float* states, const uint8_t* done, void* dgate,
-                     void* dx, float* dh0, int64_t T, int64_t E, int64_t H,
-                     int64_t gate_t, int64_t gate_e, int64_t x_t, int64_t x_e,
-                     int64_t dhs_t, int64_t dhs_e, int type);
+                     void* dx, float* dh0, float* scratch, int64_t T,
+                     int64_t E, int64_t H, int64_t gate_t, int64_t gate_e,
+                     int64_t x_t, int64_t x_e, int64_t dhs_t, int64_t dhs_e,
+                     int type);
 int rlsched_scan_step(int device, void* stream, const void* gate,
                       const void* x, const uint8_t* done, float* h, void* hs,
                       int64_t E, int64_t H, int64_t gate_e, int64_t x_e,

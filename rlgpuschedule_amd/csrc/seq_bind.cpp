@@ -29,8 +29,7 @@ using MaybeTensor = std::optional<Tensor>;
 
 namespace {
 
-constexpr int64_t kKeep = 64;      // gated_scan.hip
-constexpr int64_t kMaxTopK = 64;   // logprob.hip
+constexpr int64_t kMaxTopK = 64;  // logprob.hip
 
 template <typename E, typename... A>
 [[noreturn]] void fail(const A&... a) {
@@ -109,8 +108,11 @@ std::pair<Tensor, int64_t> rows_of(const Tensor& t) {
   return {r, r.stride(0)};
 }
 
-Tensor unit_stride(const Tensor& t) {
-  return t.size(-1) == 1 || t.stride(-1) == 1 ? t : t.contiguous();
+// t [..., E, H] with neighbouring columns and environments within reach.
+Tensor reachable(const Tensor& t) {
+  const bool near = t.stride(-2) <= rlsched_scan_reach(t.size(-1));
+  const bool unit = t.size(-1) == 1 || t.stride(-1) == 1;
+  return near && unit ? t : t.contiguous();
 }
 
 bool wants_grad(const Tensor& t) { return t.requires_grad(); }
@@ -346,8 +348,6 @@ int check_scan(const Tensor& gate, const Tensor& x, const MaybeTensor& h,
   return code;
 }
 
-int64_t kept_states(int64_t T) { return (T + kKeep - 1) / kKeep; }
-
 std::tuple<Tensor, Tensor, Tensor> scan_fwd(const Tensor& gate_,
                                             const Tensor& x_,
                                             const MaybeTensor& h0_,
@@ -358,16 +358,18 @@ std::tuple<Tensor, Tensor, Tensor> scan_fwd(const Tensor& gate_,
   const int64_t T = x_.size(0), E = x_.size(1), H = x_.size(2);
   Tensor hs = at::empty({T, E, H}, x_.options().requires_grad(false));
   Tensor h_last = f32(x_, {E, H}), states;
-  if (keep) states = f32(x_, {kept_states(T), E, H});
-  const Tensor gate = unit_stride(gate_), x = unit_stride(x_);
+  if (keep) states = f32(x_, {rlsched_scan_states(T), E, H});
+  Tensor scratch;
+  if (const int64_t n = rlsched_scan_scratch(T, E, H)) scratch = f32(x_, {n});
+  const Tensor gate = reachable(gate_), x = reachable(x_);
   const MaybeTensor h0 = packed(h0_), done = packed(done_);
   const Place at(x);
   done_with(
       rlsched_scan_fwd(at.device, at.stream, gate.const_data_ptr(),
                        x.const_data_ptr(), (const float*)ptr(h0),
                        (const uint8_t*)ptr(done), out_ptr(hs),
-                       f32_ptr(h_last), f32_ptr(states), T, E, H,
-                       gate.stride(0), gate.stride(1), x.stride(0),
+                       f32_ptr(h_last), f32_ptr(states), f32_ptr(scratch), T,
+                       E, H, gate.stride(0), gate.stride(1), x.stride(0),
                        x.stride(1), type),
       "rlsched_scan_fwd");
   return {hs, h_last, states};
@@ -386,7 +388,7 @@ std::tuple<Tensor, Tensor, Tensor> scan_bwd(
                 dhs_->scalar_type());
     same_device(x_, *dhs_, "dhs");
   }
-  VALUE_CHECK(states.dim() == 3 && states.size(0) == kept_states(T) &&
+  VALUE_CHECK(states.dim() == 3 && states.size(0) == rlsched_scan_states(T) &&
                   states.size(1) == E && states.size(2) == H &&
                   states.is_contiguous() && states.scalar_type() == at::kFloat,
               "states must be gated_scan_fwd's, of these inputs");
@@ -396,9 +398,11 @@ std::tuple<Tensor, Tensor, Tensor> scan_bwd(
   Tensor dgate = at::empty({T, E, H}, like_x);
   Tensor dx = at::empty({T, E, H}, like_x), dh0;
   if (need_dh0) dh0 = f32(x_, {E, H});
-  const Tensor gate = unit_stride(gate_), x = unit_stride(x_);
+  Tensor scratch;
+  if (const int64_t n = rlsched_scan_scratch(T, E, H)) scratch = f32(x_, {n});
+  const Tensor gate = reachable(gate_), x = reachable(x_);
   MaybeTensor dhs;
-  if (dhs_) dhs = unit_stride(*dhs_);
+  if (dhs_) dhs = reachable(*dhs_);
   const MaybeTensor dh_last = packed(dh_last_), done = packed(done_);
   const Place at(x);
   done_with(
@@ -406,8 +410,9 @@ std::tuple<Tensor, Tensor, Tensor> scan_bwd(
                        (const float*)ptr(dh_last), gate.const_data_ptr(),
                        x.const_data_ptr(), states.const_data_ptr<float>(),
                        (const uint8_t*)ptr(done), out_ptr(dgate), out_ptr(dx),
-                       f32_ptr(dh0), T, E, H, gate.stride(0), gate.stride(1),
-                       x.stride(0), x.stride(1), dhs ? dhs->stride(0) : 0,
+                       f32_ptr(dh0), f32_ptr(scratch), T, E, H,
+                       gate.stride(0), gate.stride(1), x.stride(0),
+                       x.stride(1), dhs ? dhs->stride(0) : 0,
                        dhs ? dhs->stride(1) : 0, type),
       "rlsched_scan_bwd");
   return {dgate, dx, dh0};
@@ -464,7 +469,7 @@ Tensor scan_step(const Tensor& gate_, const Tensor& x_, Tensor h,
   on_gpu(x_, "x");
   const int64_t E = x_.size(0), H = x_.size(1);
   Tensor hs = at::empty({E, H}, x_.options().requires_grad(false));
-  const Tensor gate = unit_stride(gate_), x = unit_stride(x_);
+  const Tensor gate = reachable(gate_), x = reachable(x_);
   const MaybeTensor done = packed(done_);
   const Place at(x);
   done_with(rlsched_scan_step(at.device, at.stream, gate.const_data_ptr(),
