@@ -10,7 +10,7 @@ int rlsched_norm_fwd(int device, void* stream, const void* x, const void* w,
                      const void* b, void* y, float* mean, float* rstd,
                      int64_t rows, int64_t dim, int64_t x_stride, double eps,
                      int type, int wtype);
-int64_t rlsched_norm_parts(int64_t rows, int64_t dim);
+int64_t rlsched_norm_parts(int64_t rows, int64_t dim, int type);
 int rlsched_norm_bwd(int device, void* stream, const void* dy, const void* x,
                      const void* w, const float* mean, const float* rstd,
                      void* dx, void* dw, void* db, float* partial,

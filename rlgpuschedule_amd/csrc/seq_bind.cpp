@@ -260,7 +260,7 @@ std::tuple<Tensor, Tensor, Tensor> norm_bwd(
   if (need_dw) dw = at::empty({d}, like_x.dtype(wt));
   if (need_db) db = at::empty({d}, like_x.dtype(wt));
   if (need_dw || need_db)
-    partial = f32(x, {2 * rlsched_norm_parts(rows, d) * d});
+    partial = f32(x, {2 * rlsched_norm_parts(rows, d, t.x) * d});
   const auto [xr, xs] = rows_of(x);
   const auto [dyr, dys] = rows_of(dy);
   const MaybeTensor w = packed(weight);

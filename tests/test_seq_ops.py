@@ -94,7 +94,7 @@ def norm_64(x, w, b, eps, dy=None):
 
 NORM_SIZES = [(1, 1), (3, 2), (5, 17), (64, 64), (7, 84), (33, 100),
               (130, 256), (9, 263), (4, 1000), (17, 1021), (3, 2048),
-              (2, 4096), (3, 5001), (2, 8192), (2, 16392), (1, 40001),
+              (2, 4096), (3, 5001), (2, 8192), (3, 8200), (2, 16392), (1, 40001),
               (700, 24), (2100, 256)]
 
 
