@@ -46,7 +46,7 @@ constexpr int kVec = 16 / sizeof(T);
 constexpr float kFloor = -1e4f;  // e^kFloor is 0, and so is kFloor e^kFloor
 
 // Whole numbers in the order of (value, lowest index first); 0 is nothing.
-__device__ __forceinline__ uint64_t key_of(float v, int64_t i) {
+__device__ __forceinline__ uint64_t key_of(float v, int i) {
   uint32_t b = __float_as_uint(v + 0.f);
   b = b & 0x80000000u ? ~b : b | 0x80000000u;
   return (uint64_t)b << 32 | (0xffffffffu - (uint32_t)i);
@@ -58,44 +58,53 @@ __device__ __forceinline__ float value_of(uint64_t key) {
 __device__ __forceinline__ int64_t index_of(uint64_t key) {
   return (int64_t)(0xffffffffu - (uint32_t)key);
 }
+// Vector j of a row. The last vector of a row of no whole number of them
+// begins early enough to end with the row; what it shares with the one
+// before is left out unless SHARED, so no element is counted twice.
+template <typename T>
+struct Piece {
+  Vec<T, kVec<T>> x;
+  Vec<uint8_t, kVec<T>> ok;
+  int from, skip;
 
-// Vector j of a row as floats, -inf where nothing is or may be taken. The
-// last vector of a row of no whole number of them begins early enough to end
-// with the row; what it shares with the one before is left out unless
-// `shared`, so no element is counted twice.
-template <typename T, bool shared = false>
-__device__ __forceinline__ int64_t load_row(const T* x, const uint8_t* ok,
-                                            int64_t A, int64_t j,
-                                            float (&f)[kVec<T>]) {
-  constexpr int V = kVec<T>;
-  const int64_t base = j * V;
-  int64_t from = base;
-  if (A >= V) {
-    from = base < A - V ? base : A - V;
-    load<T, V>(x + from, f);
-    if (ok) {
-      const Vec<uint8_t, V> m = load<uint8_t, V>(ok + from);
+  __device__ __forceinline__ void read(const T* row, const uint8_t* mask,
+                                       int A, int j) {
+    constexpr int V = kVec<T>;
+    const int base = j * V;
+    from = A < V || base < A - V ? base : A - V;
+    skip = base - from;
+    if (A >= V) {
+      x = load<T, V>(row + from);
+      if (mask) ok = load<uint8_t, V>(mask + from);
+    } else {
 #pragma unroll
-      for (int e = 0; e < V; ++e)
-        if (!m.v[e]) f[e] = -INFINITY;
-    }
-    if (!shared && from != base) {
-#pragma unroll
-      for (int e = 0; e < V; ++e)
-        if (from + e < base) f[e] = -INFINITY;
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      f[e] = -INFINITY;
-      if (e < A && !(ok && !ok[e])) f[e] = (float)x[e];
+      for (int e = 0; e < V; ++e) {
+        x.v[e] = e < A ? row[e] : (T)-INFINITY;
+        if (mask) ok.v[e] = e < A ? mask[e] : 0;
+      }
     }
   }
-  return from;
-}
+  // its logits, -inf where nothing may be taken
+  template <bool SHARED = false>
+  __device__ __forceinline__ void values(bool masked,
+                                         float (&f)[kVec<T>]) const {
+#pragma unroll
+    for (int e = 0; e < kVec<T>; ++e) f[e] = (float)x.v[e];
+    if (masked) {
+#pragma unroll
+      for (int e = 0; e < kVec<T>; ++e)
+        if (!ok.v[e]) f[e] = -INFINITY;
+    }
+    if (!SHARED && skip) {
+#pragma unroll
+      for (int e = 0; e < kVec<T>; ++e)
+        if (e < skip) f[e] = -INFINITY;
+    }
+  }
+};
 
 template <typename T>
-__device__ __forceinline__ void store_row(T* y, int64_t A, int64_t from,
+__device__ __forceinline__ void store_row(T* y, int A, int from,
                                           const float (&g)[kVec<T>]) {
   constexpr int V = kVec<T>;
   if (A >= V) {
@@ -112,14 +121,14 @@ __device__ __forceinline__ void store_row(T* y, int64_t A, int64_t from,
 __device__ __forceinline__ void finish_row(const LogpFwd& p, int64_t row,
                                            int64_t act, float q, float m,
                                            float s, float u) {
-  const bool broken = s != s, some = s > 0.f;
-  const float ls = some || broken ? logf(s) : 0.f;
-  const float H = some || broken ? ls - u / s : 0.f;
-  const float lp = some || broken ? q - m - ls : -INFINITY;
+  const bool any = !(s <= 0.f);  // NaN: a broken row
+  const float ls = any ? logf(s) : 0.f;
+  const float H = any ? ls - u / s : 0.f;
+  const float lp = any ? q - m - ls : -INFINITY;
   p.logp[row] = act < 0 ? 0.f : lp;
   p.entropy[row] = H;
   if (p.stats) {
-    p.stats[3 * row] = some || broken ? m : 0.f;
+    p.stats[3 * row] = any ? m : 0.f;
     p.stats[3 * row + 1] = ls;
     p.stats[3 * row + 2] = H;
   }
@@ -148,50 +157,116 @@ __device__ __forceinline__ float taken(const T* x, const uint8_t* ok,
 // What the gradient of one row's elements needs.
 struct Row {
   float m, ls, H, dl, dh;
-  int64_t act;
+  int act;
 };
 
 template <typename T>
 __device__ __forceinline__ Row row_of(const LogpBwd& p, const T* x,
                                       const uint8_t* ok, int64_t row) {
   Row r;
-  r.act = p.actions[row];
+  const int64_t act = p.actions[row];
+  r.act = (int)act;
   r.m = p.stats[3 * row];
   r.ls = p.stats[3 * row + 1];
   r.H = p.stats[3 * row + 2];
   r.dl = p.dlogp ? p.dlogp[row] : 0.f;
   r.dh = p.dentropy ? p.dentropy[row] : 0.f;
   // a taken action of probability 0 is a constant -inf
-  if (taken(x, ok, p.A, r.act) == -INFINITY) r.dl = 0.f;
+  if (taken(x, ok, p.A, act) == -INFINITY) r.dl = 0.f;
   return r;
 }
 
-__device__ __forceinline__ float gradient(const Row& r, float v, int64_t i) {
+__device__ __forceinline__ float gradient(const Row& r, float v, int i) {
   const float d = maximum(v - r.m, kFloor) - r.ls, pr = __expf(d);
   const float g = -pr * (r.dl + r.dh * (d + r.H));
   return v == -INFINITY ? 0.f : i == r.act ? g + r.dl : g;
 }
 
-// ---- rows of up to 64 * N vectors: G lanes a row, all of it in registers
-template <typename T, int G, int N>
+// How many of n keys are larger; reads of several in flight, up to kAhead
+// keys behind the last, which are not counted.
+constexpr int kAhead = 7;
+
+__device__ __forceinline__ int rank_of(uint64_t mine, const uint64_t* keys,
+                                       int n) {
+  int rank = 0;
+  for (int i = 0; i < n; i += 8) {
+    uint64_t k[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) k[j] = keys[i + j];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) rank += (k[j] > mine) & (i + j < n);
+  }
+  return rank;
+}
+
+// ---- rows of up to G * N vectors: G lanes a row, all of it in registers
+__device__ __forceinline__ uint64_t larger(uint64_t a, uint64_t b) {
+  return a > b ? a : b;
+}
+
+// A lower bound of the k-th largest element, from 64 lanes' or groups' bests,
+// no element the best of two: the least that fewer than k are above. At least
+// the lowest finite value. For one wave; the result is in all its lanes.
+__device__ __forceinline__ float least_of(const float* heads, int k) {
+  const float mine = heads[threadIdx.x % kWave];
+  int above = 0;
+#pragma unroll
+  for (int i = 0; i < kWave; ++i) above += heads[i] > mine;
+  const float least = -group_max(above < k ? -mine : -INFINITY);
+  return fmaxf(least, -3.402823466e38f);
+}
+
+// The largest of a lane's logits, and where it is first.
+template <int N, int V>
+__device__ __forceinline__ float first_best(const float (&f)[N][V],
+                                            int& slot) {
+  float top = -INFINITY;
+  slot = 0;
+#pragma unroll
+  for (int i = 0; i < N * V; ++i)
+    if (f[i / V][i % V] > top) top = f[i / V][i % V], slot = i;
+  return top;
+}
+
+template <int N, int V>
+__device__ __forceinline__ void take_out(float (&f)[N][V], int slot) {
+#pragma unroll
+  for (int i = 0; i < N * V; ++i)
+    f[i / V][i % V] = i == slot ? -INFINITY : f[i / V][i % V];
+}
+
+// The key of the at-th logit of lane l, of lanes with every G-th vector.
+template <typename T, int G>
+__device__ __forceinline__ uint64_t key_at(float v, int l, int at, int A) {
+  constexpr int V = kVec<T>;
+  const int base = (l + G * (at / V)) * V;
+  const int from = A < V || base < A - V ? base : A - V;
+  return v > -INFINITY ? key_of(v, from + at % V) : 0;
+}
+
+template <typename T, int G, int N, bool TOP>
 __global__ __launch_bounds__(256) void logp_group_kernel(LogpFwd p) {
   constexpr int V = kVec<T>, R = 256 / G;
-  const int l = threadIdx.x % G;
+  const int l = threadIdx.x % G, A = (int)p.A;
   for (int64_t row = (int64_t)blockIdx.x * R + threadIdx.x / G; row < p.rows;
        row += (int64_t)gridDim.x * R) {
     const T* x = (const T*)p.logits + row * p.x_stride;
     const uint8_t* ok = p.mask ? p.mask + row * p.mask_stride : nullptr;
     const int64_t act = p.actions[row];
+    Piece<T> piece[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if ((l + G * i) * V < A) piece[i].read(x, ok, A, l + G * i);
+    const float q = taken(x, ok, A, act);
     float f[N][V], m = -INFINITY;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
 #pragma unroll
       for (int e = 0; e < V; ++e) f[i][e] = -INFINITY;
-      if ((l + G * i) * V < p.A) load_row<T>(x, ok, p.A, l + G * i, f[i]);
+      if ((l + G * i) * V < A) piece[i].values(ok, f[i]);
 #pragma unroll
       for (int e = 0; e < V; ++e) m = maximum(m, f[i][e]);
     }
-    const float q = taken(x, ok, p.A, act);
     m = group_max<G>(m);
     if (m == -INFINITY) m = 0.f;
     float s = 0.f, u = 0.f;
@@ -206,25 +281,14 @@ __global__ __launch_bounds__(256) void logp_group_kernel(LogpFwd p) {
     s = group_sum<G>(s);
     u = group_sum<G>(u);
     if (l == 0) finish_row(p, row, act, q, m, s, u);
-    uint64_t last = ~0ull;
+    if constexpr (!TOP) continue;
+    // a round an alternative; the one found is taken out
     for (int j = 0; j < p.k; ++j) {
-      uint64_t best = 0;
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const int64_t base = (int64_t)(l + G * i) * V;
-        const int64_t from = p.A < V || base < p.A - V ? base : p.A - V;
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          const uint64_t key = key_of(f[i][e], from + e);
-          if (f[i][e] > -INFINITY && key < last && key > best) best = key;
-        }
-      }
-#pragma unroll
-      for (int o = G / 2; o > 0; o >>= 1) {
-        const uint64_t other = __shfl_xor((unsigned long long)best, o, kWave);
-        best = other > best ? other : best;
-      }
-      last = best;
+      int slot;
+      const float top = first_best(f, slot);
+      const uint64_t own = key_at<T, G>(top, l, slot, A);
+      const uint64_t best = group_larger<G>(own);
+      if (own == best) take_out(f, slot);
       if (l == 0) finish_top(p, row, j, best, m, s);
     }
   }
@@ -233,50 +297,51 @@ __global__ __launch_bounds__(256) void logp_group_kernel(LogpFwd p) {
 template <typename T, int G, int N>
 __global__ __launch_bounds__(256) void logp_group_bwd_kernel(LogpBwd p) {
   constexpr int V = kVec<T>, R = 256 / G;
-  const int l = threadIdx.x % G;
+  const int l = threadIdx.x % G, A = (int)p.A;
   for (int64_t row = (int64_t)blockIdx.x * R + threadIdx.x / G; row < p.rows;
        row += (int64_t)gridDim.x * R) {
     const T* x = (const T*)p.logits + row * p.x_stride;
     const uint8_t* ok = p.mask ? p.mask + row * p.mask_stride : nullptr;
+    T* out = (T*)p.dlogits + row * p.A;
+    Piece<T> piece[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if ((l + G * i) * V < A) piece[i].read(x, ok, A, l + G * i);
     const Row r = row_of(p, x, ok, row);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      if ((l + G * i) * V >= p.A) break;
+      if ((l + G * i) * V >= A) continue;
       float f[V];
-      const int64_t from = load_row<T, true>(x, ok, p.A, l + G * i, f);
+      piece[i].template values<true>(ok, f);
 #pragma unroll
-      for (int e = 0; e < V; ++e) f[e] = gradient(r, f[e], from + e);
-      store_row<T>((T*)p.dlogits + row * p.A, p.A, from, f);
+      for (int e = 0; e < V; ++e) f[e] = gradient(r, f[e], piece[i].from + e);
+      store_row<T>(out, A, piece[i].from, f);
     }
   }
 }
 
-// ---- longer rows, forward: W waves a row, one pass over it
+// ---- longer rows, forward: a block of 256 lanes a row, or a part of one
 // A lane's running maximum, sum and weighted sum. m starts at the lowest
 // finite value, so differences of it are never -inf minus -inf.
 struct Running {
   float m = -3.402823466e38f, s = 0.f, u = 0.f;
 
-  template <int N>
-  __device__ __forceinline__ void take(const float (&f)[N], float top) {
-    const float n = maximum(m, top);
-    const float d0 = maximum(m - n, kFloor), w0 = __expf(d0);
-    u = w0 * (u + d0 * s);
-    s = w0 * s;
-    m = n;
-#pragma unroll
-    for (int e = 0; e < N; ++e) {
-      const float d = maximum(f[e] - m, kFloor), w = __expf(d);
-      s += w;
-      u += w * d;
-    }
-  }
   // as they would be below a larger maximum
   __device__ __forceinline__ void lower(float n) {
     const float d0 = maximum(m - n, kFloor), w0 = __expf(d0);
     u = w0 * (u + d0 * s);
     s = w0 * s;
     m = n;
+  }
+  template <int N>
+  __device__ __forceinline__ void take(const float (&f)[N], float top) {
+    lower(maximum(m, top));
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const float d = maximum(f[e] - m, kFloor), w = __expf(d);
+      s += w;
+      u += w * d;
+    }
   }
   __device__ __forceinline__ void join_wave() {
     lower(group_max(m));
@@ -285,162 +350,358 @@ struct Running {
   }
 };
 
-constexpr int kHeads = 128;   // groups of lanes whose best bound the top k
-constexpr int kFound = 1024;  // alternatives that are sorted out at once
+constexpr int kLanes = 256;
+constexpr int kFound = 256;  // alternatives that are sorted out at once
 
-template <int NT>
-struct RowLds {
-  float m[NT / kWave], s[NT / kWave], u[NT / kWave];
-  uint64_t heads[kHeads];
-  uint64_t found[kFound];
-  uint64_t bound;
-  int count;
+// least_of a block's lanes, four of which have a head. `count` is cleared.
+__device__ __forceinline__ float block_least(float own, int k, float* heads,
+                                             float* at, int* count) {
+  const float head = group_max<4>(own);
+  if (threadIdx.x % 4 == 0) heads[threadIdx.x / 4] = head;
+  __syncthreads();
+  if (threadIdx.x < kWave) {
+    const float least = least_of(heads, k);
+    if (threadIdx.x == 0) *at = least, *count = 0;
+  }
+  __syncthreads();
+  return *at;
+}
+
+// The largest of a block's keys; `keys` has one for each wave.
+__device__ __forceinline__ uint64_t block_larger(uint64_t k, uint64_t* keys) {
+  k = group_larger(k);
+  if (threadIdx.x % kWave == 0) keys[threadIdx.x / kWave] = k;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kLanes / kWave; ++i) k = larger(k, keys[i]);
+  __syncthreads();
+  return k;
+}
+
+// The parts of a row that blocks of their own have seen: (m, s, u) of each,
+// and its k best keys in their order, zeros behind the last.
+struct Parts {
+  float* sums;     // [rows, parts, 3]
+  uint64_t* keys;  // [rows, parts, k]
+  int parts;       // of each row; 1: the block writes the row's results
 };
 
-template <typename T, int NT, bool TOP>
-__global__ __launch_bounds__(NT) void logp_row_kernel(LogpFwd p) {
-  constexpr int V = kVec<T>, W = NT / kWave, U = 4;
-  __shared__ RowLds<NT> lds;
+template <typename T, bool TOP>
+__global__ __launch_bounds__(kLanes) void logp_row_kernel(LogpFwd p,
+                                                          Parts parts) {
+  constexpr int V = kVec<T>, W = kLanes / kWave, U = 4;
+  __shared__ float sums[3][W], heads[kWave], least_at;
+  __shared__ uint64_t found[kFound + kAhead], waves[W];
+  __shared__ int count_at;
   const int tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave;
-  const int64_t n = (p.A + V - 1) / V;
-  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
+  const int A = (int)p.A, all = (A + V - 1) / V, P = parts.parts;
+  for (int64_t b = blockIdx.x; b < p.rows * P; b += gridDim.x) {
+    const int64_t row = P == 1 ? b : b / P;
+    const int part = P == 1 ? 0 : (int)(b - row * P);
+    const int first = (int)((int64_t)all * part / P);
+    const int n = (int)((int64_t)all * (part + 1) / P);
     const T* x = (const T*)p.logits + row * p.x_stride;
     const uint8_t* ok = p.mask ? p.mask + row * p.mask_stride : nullptr;
-    const int64_t act = p.actions[row];
-    const float q = taken(x, ok, p.A, act);
     Running r;
-    int64_t best = -1;  // the first vector that holds the lane's maximum
-    auto take = [&](const float(&f)[V], int64_t j) {
+    float own = -INFINITY;
+    auto take = [&](const Piece<T>& v) {
+      float f[V];
+      v.values(ok, f);
       float top = f[0];
 #pragma unroll
       for (int e = 1; e < V; ++e) top = maximum(top, f[e]);
-      if (TOP && (top > r.m || (best < 0 && top > -INFINITY))) best = j;
+      if (TOP) own = maximum(own, top);
       r.take(f, top);
     };
-    int64_t j = tid;
-    for (; j + (U - 1) * NT < n; j += U * NT) {
-      float f[U][V];
+    int j = first + tid;
+    for (; j + (U - 1) * kLanes < n; j += U * kLanes) {
+      Piece<T> v[U];
 #pragma unroll
-      for (int i = 0; i < U; ++i) load_row<T>(x, ok, p.A, j + i * NT, f[i]);
+      for (int i = 0; i < U; ++i) v[i].read(x, ok, A, j + i * kLanes);
 #pragma unroll
-      for (int i = 0; i < U; ++i) take(f[i], j + i * NT);
+      for (int i = 0; i < U; ++i) take(v[i]);
     }
-    for (; j < n; j += NT) {
-      float f[V];
-      load_row<T>(x, ok, p.A, j, f);
-      take(f, j);
+    for (; j < n; j += kLanes) {
+      Piece<T> v;
+      v.read(x, ok, A, j);
+      take(v);
     }
-    const float own = r.m;
     r.join_wave();
     if (lane == 0) {
-      lds.m[wave] = r.m;
-      lds.s[wave] = r.s;
-      lds.u[wave] = r.u;
+      sums[0][wave] = r.m;
+      sums[1][wave] = r.s;
+      sums[2][wave] = r.u;
     }
     __syncthreads();
-    float m = lds.m[0], s = 0.f, u = 0.f;
+    float m = sums[0][0], s = 0.f, u = 0.f;
 #pragma unroll
-    for (int i = 1; i < W; ++i) m = maximum(m, lds.m[i]);
+    for (int i = 1; i < W; ++i) m = maximum(m, sums[0][i]);
 #pragma unroll
     for (int i = 0; i < W; ++i) {
-      Running part{lds.m[i], lds.s[i], lds.u[i]};
-      part.lower(m);
-      s += part.s;
-      u += part.u;
+      Running one{sums[0][i], sums[1][i], sums[2][i]};
+      one.lower(m);
+      s += one.s;
+      u += one.u;
     }
-    if (tid == 0) finish_row(p, row, act, q, m, s, u);
+    if (tid == 0) {
+      if (P == 1) {
+        const int64_t act = p.actions[row];
+        finish_row(p, row, act, taken(x, ok, A, act), m, s, u);
+      } else {
+        parts.sums[3 * b] = m;
+        parts.sums[3 * b + 1] = s;
+        parts.sums[3 * b + 2] = u;
+      }
+    }
     if (TOP) {
-      // Each of kHeads groups of lanes has its best; the k-th of those is a
-      // lower bound of the k-th of all, and only lanes whose own best
-      // reaches it have more to give: about k elements, at most k groups'.
-      uint64_t key = 0;
-      if (best >= 0 && s == s) {
-        float f[V];
-        const int64_t from = load_row<T>(x, ok, p.A, best, f);
+      auto put = [&](int i, uint64_t key) {
+        if (P == 1) {
+          finish_top(p, row, i, key, m, s);
+        } else {
+          parts.keys[b * p.k + i] = key;
+        }
+      };
+      // only lanes whose own best reaches the bound have more to give
+      const float least =
+          block_least(own, p.k, heads, &least_at, &count_at);
+      if (own >= least) {
+        for (int i = first + tid; i < n; i += U * kLanes) {
+          Piece<T> v[U];
 #pragma unroll
-        for (int e = V - 1; e >= 0; --e)
-          if (f[e] == own) key = key_of(f[e], from + e);
-      }
-      uint64_t head = key;
+          for (int c = 0; c < U; ++c)
+            if (i + c * kLanes < n) v[c].read(x, ok, A, i + c * kLanes);
 #pragma unroll
-      for (int o = 1; o < NT / kHeads; o <<= 1) {
-        const uint64_t other = __shfl_xor((unsigned long long)head, o, kWave);
-        head = other > head ? other : head;
-      }
-      if (tid % (NT / kHeads) == 0) lds.heads[tid / (NT / kHeads)] = head;
-      if (tid == 0) {
-        lds.bound = 1;
-        lds.count = 0;
-      }
-      __syncthreads();
-      if (tid < kHeads) {
-        const uint64_t mine = lds.heads[tid];
-        int rank = 0;
-        for (int i = 0; i < kHeads; ++i) rank += lds.heads[i] > mine;
-        if (mine && rank == p.k - 1) lds.bound = mine;
-      }
-      __syncthreads();
-      const uint64_t bound = lds.bound;
-      if (key >= bound) {
-        for (int64_t i = tid; i < n; i += NT) {
-          float f[V];
-          const int64_t from = load_row<T>(x, ok, p.A, i, f);
+          for (int c = 0; c < U; ++c) {
+            if (i + c * kLanes >= n) continue;
+            float f[V];
+            v[c].values(ok, f);
 #pragma unroll
-          for (int e = 0; e < V; ++e) {
-            const uint64_t k = key_of(f[e], from + e);
-            if (f[e] > -INFINITY && k >= bound) {
-              const int at = atomicAdd(&lds.count, 1);
-              if (at < kFound) lds.found[at] = k;
+            for (int e = 0; e < V; ++e) {
+              if (!(f[e] >= least)) continue;
+              const int at = atomicAdd(&count_at, 1);
+              if (at < kFound) found[at] = key_of(f[e], v[c].from + e);
             }
           }
         }
       }
       __syncthreads();
-      const int count = lds.count;
+      const int count = count_at;
       if (count <= kFound) {
-        for (int i = tid; i < count; i += NT) {
-          const uint64_t mine = lds.found[i];
-          int rank = 0;
-          for (int c = 0; c < count; ++c) rank += lds.found[c] > mine;
-          if (rank < p.k) finish_top(p, row, rank, mine, m, s);
+        // whatever order they were found in, each goes to its rank
+        for (int i = tid; i < count; i += kLanes) {
+          const uint64_t mine = found[i];
+          const int rank = rank_of(mine, found, count);
+          if (rank < p.k) put(rank, mine);
         }
-        for (int i = count + tid; i < p.k; i += NT)
-          finish_top(p, row, i, 0, m, s);
+        for (int i = count + tid; i < p.k; i += kLanes) put(i, 0);
       } else {
-        // More than fit: few lanes hold many of the largest. One round an
-        // alternative, each a maximum below the one before.
+        // More than fit, such as many equal ones: one round an alternative,
+        // each a maximum below the one before.
         uint64_t last = ~0ull;
         for (int a = 0; a < p.k; ++a) {
           uint64_t top = 0;
-          if (key >= bound) {
-            for (int64_t i = tid; i < n; i += NT) {
+          if (own >= least) {
+            for (int i = first + tid; i < n; i += kLanes) {
+              Piece<T> v;
+              v.read(x, ok, A, i);
               float f[V];
-              const int64_t from = load_row<T>(x, ok, p.A, i, f);
+              v.values(ok, f);
 #pragma unroll
               for (int e = 0; e < V; ++e) {
-                const uint64_t k = key_of(f[e], from + e);
+                const uint64_t k = key_of(f[e], v.from + e);
                 if (f[e] > -INFINITY && k < last && k > top) top = k;
               }
             }
           }
-#pragma unroll
-          for (int o = kWave / 2; o > 0; o >>= 1) {
-            const uint64_t other =
-                __shfl_xor((unsigned long long)top, o, kWave);
-            top = other > top ? other : top;
-          }
-          if (lane == 0) lds.heads[wave] = top;
-          __syncthreads();
-#pragma unroll
-          for (int i = 0; i < W; ++i)
-            top = lds.heads[i] > top ? lds.heads[i] : top;
-          __syncthreads();
-          last = top;
-          if (tid == 0) finish_top(p, row, a, top, m, s);
+          last = block_larger(top, waves);
+          if (tid == 0) put(a, last);
         }
       }
     }
-    __syncthreads();  // the next row writes what this one reads
+    __syncthreads();  // the next turn writes what this one reads
+  }
+}
+
+// The same for parts of up to kHeld vectors with alternatives, N of them in a
+// lane's registers: nothing is read twice.
+constexpr int kHeld = 4 * kLanes;
+
+template <typename T, int N>
+__global__ __launch_bounds__(kLanes) void logp_part_kernel(LogpFwd p,
+                                                           Parts parts) {
+  constexpr int V = kVec<T>, W = kLanes / kWave;
+  __shared__ float sums[3][W], heads[kWave], least_at;
+  __shared__ uint64_t found[kFound + kAhead], waves[W];
+  __shared__ int count_at;
+  const int tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave;
+  const int A = (int)p.A, all = (A + V - 1) / V, P = parts.parts;
+  for (int64_t b = blockIdx.x; b < p.rows * P; b += gridDim.x) {
+    const int64_t row = P == 1 ? b : b / P;
+    const int part = P == 1 ? 0 : (int)(b - row * P);
+    const int first = (int)((int64_t)all * part / P);
+    const int n = (int)((int64_t)all * (part + 1) / P);
+    const T* x = (const T*)p.logits + row * p.x_stride;
+    const uint8_t* ok = p.mask ? p.mask + row * p.mask_stride : nullptr;
+    Piece<T> v[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (first + tid + i * kLanes < n)
+        v[i].read(x, ok, A, first + tid + i * kLanes);
+    float f[N][V], tops[N], top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) f[i][e] = -INFINITY;
+      if (first + tid + i * kLanes < n) v[i].values(ok, f[i]);
+      tops[i] = f[i][0];
+#pragma unroll
+      for (int e = 1; e < V; ++e) tops[i] = maximum(tops[i], f[i][e]);
+      top = maximum(top, tops[i]);
+    }
+    float m = group_max(top);
+    if (lane == 0) sums[0][wave] = m;
+    const float least =
+        block_least(top, p.k, heads, &least_at, &count_at);
+#pragma unroll
+    for (int i = 0; i < W; ++i) m = maximum(m, sums[0][i]);
+    if (m == -INFINITY) m = -3.402823466e38f;
+    float s = 0.f, u = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float d = maximum(f[i][e] - m, kFloor), w = __expf(d);
+        s += w;
+        u += w * d;
+      }
+    s = group_sum(s);
+    u = group_sum(u);
+    if (lane == 0) sums[1][wave] = s, sums[2][wave] = u;
+    auto index = [&](int at) {
+      const int base = (first + tid + at / V * kLanes) * V;
+      return (base < A - V ? base : A - V) + at % V;
+    };
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (!(tops[i] >= least)) continue;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        if (!(f[i][e] >= least)) continue;
+        const int at = atomicAdd(&count_at, 1);
+        if (at < kFound) found[at] = key_of(f[i][e], index(i * V + e));
+      }
+    }
+    __syncthreads();
+    s = u = 0.f;
+#pragma unroll
+    for (int i = 0; i < W; ++i) s += sums[1][i], u += sums[2][i];
+    if (tid == 0) {
+      if (P == 1) {
+        const int64_t act = p.actions[row];
+        finish_row(p, row, act, taken(x, ok, A, act), m, s, u);
+      } else {
+        parts.sums[3 * b] = m;
+        parts.sums[3 * b + 1] = s;
+        parts.sums[3 * b + 2] = u;
+      }
+    }
+    auto put = [&](int i, uint64_t key) {
+      if (P == 1) {
+        finish_top(p, row, i, key, m, s);
+      } else {
+        parts.keys[b * p.k + i] = key;
+      }
+    };
+    const int count = count_at;
+    if (count <= kFound) {
+      // whatever order they were found in, each goes to its rank
+      for (int i = tid; i < count || i < p.k; i += kLanes) {
+        const uint64_t mine = i < count ? found[i] : 0;
+        const int at = i < count ? rank_of(mine, found, count) : i;
+        if (at < p.k) put(at, mine);
+      }
+    } else {
+      // many equal ones: a round an alternative, and it is taken out
+      for (int j = 0; j < p.k; ++j) {
+        int slot;
+        const float best = first_best(f, slot);
+        const uint64_t own =
+            best > -INFINITY ? key_of(best, index(slot)) : 0;
+        const uint64_t key = block_larger(own, waves);
+        if (own == key) take_out(f, slot);
+        if (tid == 0) put(j, key);
+      }
+    }
+    __syncthreads();  // the next turn writes what this one reads
+  }
+}
+
+// The k-th largest of n keys, none of them twice but 0; 1 if there are fewer
+// than k. Whole blocks, n <= kLanes; `keys` is in LDS and complete.
+__device__ __forceinline__ uint64_t kth(const uint64_t* keys, int n, int k,
+                                        uint64_t* out) {
+  const int tid = threadIdx.x;
+  if (tid == 0) *out = 1;
+  __syncthreads();
+  if (tid < n) {
+    const uint64_t mine = keys[tid];
+    if (rank_of(mine, keys, n) == k - 1 && mine) *out = mine;
+  }
+  __syncthreads();
+  return *out;
+}
+
+// One row's results from its parts'. Of each part's sorted keys the first
+// few bound the k-th of all, and what reaches the bound goes to its rank.
+constexpr int kMostParts = 64;
+
+__global__ __launch_bounds__(kLanes) void logp_join_kernel(LogpFwd p,
+                                                           Parts parts,
+                                                           int type) {
+  __shared__ uint64_t heads[kLanes], found[kMostParts * 64 + kAhead];
+  __shared__ uint64_t bound_at;
+  __shared__ int count_at;
+  const int tid = threadIdx.x, P = parts.parts, k = p.k;
+  for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
+    const float* sums = parts.sums + 3 * row * P;
+    const int i0 = tid % kWave < P ? tid % kWave : 0;
+    Running r{sums[3 * i0], sums[3 * i0 + 1], sums[3 * i0 + 2]};
+    if (tid % kWave >= P) r.s = r.u = 0.f;
+    r.join_wave();
+    if (tid == 0) {
+      const int64_t act = p.actions[row];
+      const uint8_t* ok = p.mask ? p.mask + row * p.mask_stride : nullptr;
+      float q;
+      if (type == F32) {
+        q = taken((const float*)p.logits + row * p.x_stride, ok, p.A, act);
+      } else if (type == BF16) {
+        q = taken((const bf16*)p.logits + row * p.x_stride, ok, p.A, act);
+      } else {
+        q = taken((const f16*)p.logits + row * p.x_stride, ok, p.A, act);
+      }
+      finish_row(p, row, act, q, r.m, r.s, r.u);
+      count_at = 0;
+    }
+    if (k == 0) continue;
+    const uint64_t* keys = parts.keys + row * P * k;
+    const int each = (k + P - 1) / P, n = P * each;  // < k + P
+    if (tid < n) heads[tid] = keys[tid / each * k + tid % each];
+    __syncthreads();
+    const uint64_t bound = kth(heads, n, k, &bound_at);
+    for (int i = tid; i < P * k; i += kLanes) {
+      const uint64_t key = keys[i];
+      if (key >= bound) found[atomicAdd(&count_at, 1)] = key;
+    }
+    __syncthreads();
+    const int count = count_at;
+    for (int i = tid; i < count; i += kLanes) {
+      const uint64_t mine = found[i];
+      const int rank = rank_of(mine, found, count);
+      if (rank < k) finish_top(p, row, rank, mine, r.m, r.s);
+    }
+    for (int i = count + tid; i < k; i += kLanes)
+      finish_top(p, row, i, 0, r.m, r.s);
+    __syncthreads();
   }
 }
 
@@ -451,81 +712,135 @@ template <typename T>
 __global__ __launch_bounds__(256) void logp_row_bwd_kernel(LogpBwd p,
                                                            int64_t pieces) {
   constexpr int V = kVec<T>, U = kBwdVecs;
-  const int64_t n = (p.A + V - 1) / V;
+  const int A = (int)p.A, n = (A + V - 1) / V;
   for (int64_t b = blockIdx.x; b < p.rows * pieces; b += gridDim.x) {
     const int64_t row = b / pieces;
-    const int64_t j = b % pieces * (256 * U) + threadIdx.x;
+    const int j = (int)(b - row * pieces) * (256 * U) + threadIdx.x;
     const T* x = (const T*)p.logits + row * p.x_stride;
     const uint8_t* ok = p.mask ? p.mask + row * p.mask_stride : nullptr;
-    float f[U][V];
-    int64_t from[U];
+    T* out = (T*)p.dlogits + row * p.A;
+    Piece<T> v[U];
 #pragma unroll
     for (int i = 0; i < U; ++i)
-      if (j + 256 * i < n)
-        from[i] = load_row<T, true>(x, ok, p.A, j + 256 * i, f[i]);
+      if (j + 256 * i < n) v[i].read(x, ok, A, j + 256 * i);
     const Row r = row_of(p, x, ok, row);
 #pragma unroll
     for (int i = 0; i < U; ++i) {
       if (j + 256 * i >= n) break;
+      float f[V];
+      v[i].template values<true>(ok, f);
 #pragma unroll
-      for (int e = 0; e < V; ++e) f[i][e] = gradient(r, f[i][e], from[i] + e);
-      store_row<T>((T*)p.dlogits + row * p.A, p.A, from[i], f[i]);
+      for (int e = 0; e < V; ++e) f[e] = gradient(r, f[e], v[i].from + e);
+      store_row<T>(out, A, v[i].from, f);
     }
   }
 }
 
-constexpr int64_t kGrid = 1 << 22;  // blocks at most; more rows are looped over
+constexpr int64_t kGrid = 1 << 22;  // blocks at most; more are looped over
 
-template <typename T, int G, int N>
-hipError_t group_fwd(const LogpFwd& p, hipStream_t s) {
-  const int64_t grid = (p.rows + 256 / G - 1) / (256 / G);
-  return launch(logp_group_kernel<T, G, N>, dim3(grid < kGrid ? grid : kGrid),
-                dim3(256), 0, s, p);
-}
-template <typename T, int G, int N>
-hipError_t group_bwd(const LogpBwd& p, hipStream_t s) {
-  const int64_t grid = (p.rows + 256 / G - 1) / (256 / G);
-  return launch(logp_group_bwd_kernel<T, G, N>,
-                dim3(grid < kGrid ? grid : kGrid), dim3(256), 0, s, p);
+// Rows that G lanes hold in registers: G as few as four vectors a lane allow.
+struct Group {
+  int G, N;
+};
+
+Group group_of(int64_t A, int V) {
+  const int64_t n = (A + V - 1) / V;
+  int G = 1;
+  while (4 * G < n) G *= 2;
+  return {G, (int)((n + G - 1) / G)};
 }
 
-template <typename T, int NT>
-hipError_t row_fwd(const LogpFwd& p, hipStream_t s) {
-  const dim3 grid(p.rows < kGrid ? p.rows : kGrid);
-  if (p.k)
-    return launch(logp_row_kernel<T, NT, true>, grid, dim3(NT), 0, s, p);
-  return launch(logp_row_kernel<T, NT, false>, grid, dim3(NT), 0, s, p);
+// Vectors of the longest row that a wave's lanes hold; with alternatives,
+// which cost a group a round each, half a wave's. Longer ones take blocks.
+constexpr int64_t group_vecs(int k) { return k ? 2 * kWave : 4 * kWave; }
+
+template <typename T, bool BWD, int G, int N, typename P>
+hipError_t group_with(const P& p, hipStream_t s) {
+  constexpr int B = 256;
+  const int64_t want = (p.rows + B / G - 1) / (B / G);
+  const dim3 grid(want < kGrid ? want : kGrid);
+  if constexpr (BWD) {
+    return launch(logp_group_bwd_kernel<T, G, N>, grid, dim3(B), 0, s, p);
+  } else {
+    if constexpr (G < kWave) {
+      if (p.k)
+        return launch(logp_group_kernel<T, G, N, true>, grid, dim3(B), 0, s,
+                      p);
+    }
+    return launch(logp_group_kernel<T, G, N, false>, grid, dim3(B), 0, s, p);
+  }
+}
+
+template <typename T, bool BWD, typename P>
+hipError_t group(const P& p, hipStream_t s) {
+  const Group g = group_of(p.A, kVec<T>);
+  switch (g.G * 8 + g.N) {
+    case 1 * 8 + 1: return group_with<T, BWD, 1, 1>(p, s);
+    case 1 * 8 + 2: return group_with<T, BWD, 1, 2>(p, s);
+    case 1 * 8 + 3: return group_with<T, BWD, 1, 3>(p, s);
+    case 1 * 8 + 4: return group_with<T, BWD, 1, 4>(p, s);
+    case 2 * 8 + 3: return group_with<T, BWD, 2, 3>(p, s);
+    case 2 * 8 + 4: return group_with<T, BWD, 2, 4>(p, s);
+    case 4 * 8 + 3: return group_with<T, BWD, 4, 3>(p, s);
+    case 4 * 8 + 4: return group_with<T, BWD, 4, 4>(p, s);
+    case 8 * 8 + 3: return group_with<T, BWD, 8, 3>(p, s);
+    case 8 * 8 + 4: return group_with<T, BWD, 8, 4>(p, s);
+    case 16 * 8 + 3: return group_with<T, BWD, 16, 3>(p, s);
+    case 16 * 8 + 4: return group_with<T, BWD, 16, 4>(p, s);
+    case 32 * 8 + 3: return group_with<T, BWD, 32, 3>(p, s);
+    case 32 * 8 + 4: return group_with<T, BWD, 32, 4>(p, s);
+    case 64 * 8 + 3: return group_with<T, BWD, 64, 3>(p, s);
+    case 64 * 8 + 4: return group_with<T, BWD, 64, 4>(p, s);
+  }
+  return hipErrorInvalidValue;
+}
+
+// Parts of a row: of 512 vectors at least, while there are fewer blocks than
+// keep the chip busy; with alternatives of as many as registers hold at most.
+int parts_of(int64_t rows, int64_t A, int k, int V) {
+  const int64_t n = (A + V - 1) / V;
+  if (n <= group_vecs(k) || rows <= 0) return 1;
+  int64_t p = (1024 + rows - 1) / rows;
+  p = p < n / 512 ? p : n / 512;
+  if (k && p < (n + kHeld - 1) / kHeld) p = (n + kHeld - 1) / kHeld;
+  p = p < kMostParts ? p : kMostParts;
+  return p < 1 ? 1 : (int)p;
 }
 
 template <typename T>
-hipError_t fwd(const LogpFwd& p, hipStream_t s) {
+hipError_t fwd(const LogpFwd& p, void* scratch, int type, hipStream_t s) {
   if (p.rows == 0) return hipSuccess;
   const int64_t n = (p.A + kVec<T> - 1) / kVec<T>;
-  if (n <= 1) return group_fwd<T, 1, 1>(p, s);
-  if (n <= 2) return group_fwd<T, 2, 1>(p, s);
-  if (n <= 4) return group_fwd<T, 4, 1>(p, s);
-  if (n <= 8) return group_fwd<T, 8, 1>(p, s);
-  if (n <= 16) return group_fwd<T, 16, 1>(p, s);
-  if (n <= 32) return group_fwd<T, 32, 1>(p, s);
-  if (n <= 64) return group_fwd<T, 64, 1>(p, s);
-  if (n <= 128) return group_fwd<T, 64, 2>(p, s);
-  if (n <= 256) return group_fwd<T, 64, 4>(p, s);
-  if (n >= 2048 && p.rows < 512) return row_fwd<T, 1024>(p, s);
-  return row_fwd<T, 256>(p, s);
+  if (n <= group_vecs(p.k)) return group<T, false>(p, s);
+  const int P = parts_of(p.rows, p.A, p.k, kVec<T>);
+  const int64_t blocks = p.rows * P;
+  const Parts parts = {(float*)((uint64_t*)scratch + blocks * p.k),
+                       (uint64_t*)scratch, P};
+  const dim3 grid(blocks < kGrid ? blocks : kGrid);
+  const dim3 lanes(kLanes);
+  hipError_t e;
+  if (p.k == 0) {
+    e = launch(logp_row_kernel<T, false>, grid, lanes, 0, s, p, parts);
+  } else if (n <= (int64_t)kLanes * P) {
+    e = launch(logp_part_kernel<T, 1>, grid, lanes, 0, s, p, parts);
+  } else if (n <= 2 * (int64_t)kLanes * P) {
+    e = launch(logp_part_kernel<T, 2>, grid, lanes, 0, s, p, parts);
+  } else if (n <= (int64_t)kHeld * P) {
+    e = launch(logp_part_kernel<T, kHeld / kLanes>, grid, lanes, 0, s, p,
+               parts);
+  } else {
+    e = launch(logp_row_kernel<T, true>, grid, lanes, 0, s, p, parts);
+  }
+  if (e != hipSuccess || P == 1) return e;
+  return launch(logp_join_kernel, dim3(p.rows < kGrid ? p.rows : kGrid),
+                dim3(kLanes), 0, s, p, parts, type);
 }
 
 template <typename T>
 hipError_t bwd(const LogpBwd& p, hipStream_t s) {
   if (p.rows == 0) return hipSuccess;
   const int64_t n = (p.A + kVec<T> - 1) / kVec<T>;
-  if (n <= 1) return group_bwd<T, 1, 1>(p, s);
-  if (n <= 2) return group_bwd<T, 2, 1>(p, s);
-  if (n <= 4) return group_bwd<T, 4, 1>(p, s);
-  if (n <= 8) return group_bwd<T, 8, 1>(p, s);
-  if (n <= 16) return group_bwd<T, 16, 1>(p, s);
-  if (n <= 32) return group_bwd<T, 32, 1>(p, s);
-  if (n <= 64) return group_bwd<T, 64, 1>(p, s);
-  if (n <= 128) return group_bwd<T, 64, 2>(p, s);
+  if (n <= group_vecs(0)) return group<T, true>(p, s);
   const int64_t pieces = (n + 256 * kBwdVecs - 1) / (256 * kBwdVecs);
   const int64_t grid = p.rows * pieces;
   return launch(logp_row_bwd_kernel<T>, dim3(grid < kGrid ? grid : kGrid),
@@ -534,20 +849,28 @@ hipError_t bwd(const LogpBwd& p, hipStream_t s) {
 
 }  // namespace
 
+// Bytes of scratch that the forward call needs.
+extern "C" int64_t rlsched_logp_scratch(int64_t rows, int64_t A, int k,
+                                        int type) {
+  const int P = parts_of(rows, A, k, type == F32 ? 4 : 8);
+  return P == 1 ? 0 : rows * P * (8 * (int64_t)k + 12);
+}
+
 extern "C" int rlsched_logp_fwd(int device, void* stream, const void* logits,
                                 const int64_t* actions, const uint8_t* mask,
                                 float* logp, float* entropy, float* stats,
                                 float* top_logp, int64_t* top_index,
-                                int64_t rows, int64_t A, int64_t x_stride,
-                                int64_t mask_stride, int k, int type) {
+                                void* scratch, int64_t rows, int64_t A,
+                                int64_t x_stride, int64_t mask_stride, int k,
+                                int type) {
   OnDevice on(device);
   if (on.err != hipSuccess) return on.err;
   const LogpFwd p = {logits, actions,  mask,      logp, entropy,  stats,
                      top_logp, top_index, rows, A, x_stride, mask_stride, k};
   const hipStream_t s = (hipStream_t)stream;
-  if (type == F32) return fwd<float>(p, s);
-  if (type == BF16) return fwd<bf16>(p, s);
-  if (type == F16) return fwd<f16>(p, s);
+  if (type == F32) return fwd<float>(p, scratch, type, s);
+  if (type == BF16) return fwd<bf16>(p, scratch, type, s);
+  if (type == F16) return fwd<f16>(p, scratch, type, s);
   return hipErrorInvalidValue;
 }
 

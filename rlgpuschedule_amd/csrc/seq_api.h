@@ -37,11 +37,13 @@ int rlsched_scan_step(int device, void* stream, const void* gate,
                       int64_t E, int64_t H, int64_t gate_e, int64_t x_e,
                       int type);
 
+int64_t rlsched_logp_scratch(int64_t rows, int64_t A, int k, int type);
 int rlsched_logp_fwd(int device, void* stream, const void* logits,
                      const int64_t* actions, const uint8_t* mask, float* logp,
                      float* entropy, float* stats, float* top_logp,
-                     int64_t* top_index, int64_t rows, int64_t A,
-                     int64_t x_stride, int64_t mask_stride, int k, int type);
+                     int64_t* top_index, void* scratch, int64_t rows,
+                     int64_t A, int64_t x_stride, int64_t mask_stride, int k,
+                     int type);
 int rlsched_logp_bwd(int device, void* stream, const float* dlogp,
                      const float* dentropy, const void* logits,
                      const int64_t* actions, const uint8_t* mask,

@@ -522,6 +522,10 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> logp_fwd(
     top_logp = f32(logits, size);
     top_index = at::empty(size, actions_.options().requires_grad(false));
   }
+  Tensor scratch;
+  if (const int64_t n = rlsched_logp_scratch(rows, A, (int)top_k, type))
+    scratch = at::empty(
+        {n}, logits.options().dtype(at::kByte).requires_grad(false));
   const auto [xr, xs] = rows_of(logits);
   Tensor mr;
   int64_t ms = 0;
@@ -533,8 +537,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> logp_fwd(
                        actions.const_data_ptr<int64_t>(),
                        mask ? (const uint8_t*)mr.const_data_ptr() : nullptr,
                        f32_ptr(logp), f32_ptr(entropy), f32_ptr(stats),
-                       f32_ptr(top_logp), (int64_t*)out_ptr(top_index), rows,
-                       A, xs, ms, (int)top_k, type),
+                       f32_ptr(top_logp), (int64_t*)out_ptr(top_index),
+                       out_ptr(scratch), rows, A, xs, ms, (int)top_k, type),
       "rlsched_logp_fwd");
   return {logp, entropy, stats, top_logp, top_index};
 }

@@ -52,18 +52,82 @@ __device__ __forceinline__ float maximum(float a, float b) {
   return __builtin_elementwise_maximum(a, b);
 }
 
-template <int W = kWave>
-__device__ __forceinline__ float group_sum(float v) {
-#pragma unroll
-  for (int o = W / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, kWave);
+// A reduction over groups of W lanes, its result in every one of them, by
+// moves between registers alone: quads, halves of a row of 16, the row, then
+// swaps of rows and of halves of the wave. A step's two operands may lie in
+// other lanes than an exclusive-or's would, but hold the same sums.
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp(uint32_t v) {
+  return __builtin_amdgcn_update_dpp(v, v, CTRL, 0xf, 0xf, false);
+}
+
+template <int W = kWave, typename Op>
+__device__ __forceinline__ uint32_t group_reduce(uint32_t v, Op op) {
+  if constexpr (W >= 2) v = op(v, dpp<0xb1>(v));   // quad 1 0 3 2
+  if constexpr (W >= 4) v = op(v, dpp<0x4e>(v));   // quad 2 3 0 1
+  if constexpr (W >= 8) v = op(v, dpp<0x141>(v));  // half mirror
+  if constexpr (W >= 16) v = op(v, dpp<0x140>(v));  // mirror
+  if constexpr (W >= 32) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = op(r[0], r[1]);
+  }
+  if constexpr (W >= 64) {
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    v = op(r[0], r[1]);
+  }
   return v;
 }
 
+// Not contracted: fused with a product before it, an addition would see one
+// lane's rounded and another's not, and the lanes' sums would differ.
+__device__ __forceinline__ float add(float a, float b) {
+#pragma clang fp contract(off)
+  return a + b;
+}
+
 template <int W = kWave>
-__device__ __forceinline__ float group_max(float v) {
-#pragma unroll
-  for (int o = W / 2; o > 0; o >>= 1) v = maximum(v, __shfl_xor(v, o, kWave));
-  return v;
+__device__ __forceinline__ float group_sum(float f) {
+  return __uint_as_float(
+      group_reduce<W>(__float_as_uint(f), [](uint32_t a, uint32_t b) {
+        return __float_as_uint(add(__uint_as_float(a), __uint_as_float(b)));
+      }));
+}
+
+template <int W = kWave>
+__device__ __forceinline__ float group_max(float f) {
+  return __uint_as_float(
+      group_reduce<W>(__float_as_uint(f), [](uint32_t a, uint32_t b) {
+        return __float_as_uint(
+            maximum(__uint_as_float(a), __uint_as_float(b)));
+      }));
+}
+
+// The largest of 64-bit keys.
+template <int W = kWave>
+__device__ __forceinline__ uint64_t group_larger(uint64_t k) {
+  auto step = [&](uint32_t lo, uint32_t hi) {
+    const uint64_t other = (uint64_t)hi << 32 | lo;
+    k = other > k ? other : k;
+  };
+  auto lo = [&] { return (uint32_t)k; };
+  auto hi = [&] { return (uint32_t)(k >> 32); };
+  if constexpr (W >= 2) step(dpp<0xb1>(lo()), dpp<0xb1>(hi()));
+  if constexpr (W >= 4) step(dpp<0x4e>(lo()), dpp<0x4e>(hi()));
+  if constexpr (W >= 8) step(dpp<0x141>(lo()), dpp<0x141>(hi()));
+  if constexpr (W >= 16) step(dpp<0x140>(lo()), dpp<0x140>(hi()));
+  if constexpr (W >= 32) {
+    const auto l = __builtin_amdgcn_permlane16_swap(lo(), lo(), false, false);
+    const auto h = __builtin_amdgcn_permlane16_swap(hi(), hi(), false, false);
+    step(l[0], h[0]);
+    step(l[1], h[1]);
+  }
+  if constexpr (W >= 64) {
+    const auto l = __builtin_amdgcn_permlane32_swap(lo(), lo(), false, false);
+    const auto h = __builtin_amdgcn_permlane32_swap(hi(), hi(), false, false);
+    step(l[0], h[0]);
+    step(l[1], h[1]);
+  }
+  return k;
 }
 
 // Runs the scope on one device and goes back to the caller's.

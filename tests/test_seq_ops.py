@@ -569,7 +569,8 @@ def check_logp(logits, actions, mask, top_k, dlogp, dent, what=""):
 
 LOGP_SIZES = [(1, 1), (3, 2), (50, 5), (300, 17), (5, 21), (70, 64), (33, 65),
               (9, 100), (4, 256), (7, 1000), (3, 1024), (5, 4097), (2, 8192),
-              (2, 10007), (1, 20000), (1, 70000), (3, 32768)]
+              (2, 10007), (1, 20000), (1, 70000), (3, 32768),
+              (2, 600007)]
 
 
 @pytest.mark.parametrize("device", DEVICES)
