@@ -66,19 +66,6 @@ struct Place {
 };
 
 template <typename T>
-__device__ __forceinline__ void load_at(const T* p, int dim,
-                                        const Place<T>& at,
-                                        float (&f)[kVec<T>]) {
-  constexpr int V = kVec<T>;
-  if (dim >= V) {
-    load<T, V>(p + at.from, f);
-  } else {
-#pragma unroll
-    for (int e = 0; e < V; ++e) f[e] = e < dim ? (float)p[e] : 0.f;
-  }
-}
-
-template <typename T>
 __device__ __forceinline__ void store_at(T* p, int dim, const Place<T>& at,
                                          const float (&f)[kVec<T>]) {
   constexpr int V = kVec<T>;
@@ -137,7 +124,7 @@ __device__ __forceinline__ void row_sum(float (&v)[K],
 }
 
 template <int G>
-constexpr int kBlock = G > kWave ? G : 256;  // rows share a block, not a barrier
+constexpr int kBlock = G > kWave ? G : 512;  // rows share a block, not a barrier
 
 template <typename T, int G, int N>
 __global__ __launch_bounds__(kBlock<G>) void norm_fwd_kernel(NormFwd p) {
@@ -145,22 +132,44 @@ __global__ __launch_bounds__(kBlock<G>) void norm_fwd_kernel(NormFwd p) {
   __shared__ float lds[2][1][G / kWave + 1];
   const int l = threadIdx.x % G, dim = (int)p.dim;
   const float over = 1.f / (float)dim;
-  for (int64_t row = (int64_t)blockIdx.x * R + threadIdx.x / G; row < p.rows;
-       row += (int64_t)gridDim.x * R) {
-    const T* x = (const T*)p.x + row * p.x_stride;
-    float f[N][V], s[1] = {0.f};
+  Vec<T, V> x[N];
+  auto read = [&](int64_t row) {
+    const T* xr = (const T*)p.x + row * p.x_stride;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const Place<T> at(dim, l + G * i);
-      if (at.some) load_at<T>(x, dim, at, f[i]);
+      if (!at.some) continue;
+      if (dim >= V) {
+        x[i] = load<T, V>(xr + at.from);
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) x[i].v[e] = e < dim ? xr[e] : (T)0.f;
+      }
     }
+  };
+  const int64_t step = (int64_t)gridDim.x * R;
+  int64_t row = (int64_t)blockIdx.x * R + threadIdx.x / G;
+  if (row < p.rows) read(row);
+  float w[N][V], b[N][V];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const Place<T> at(dim, l + G * i);
+    load_param<T>(p.w, p.w32, dim, at, 1.f, w[i]);
+    load_param<T>(p.b, p.w32, dim, at, 0.f, b[i]);
+  }
+  for (; row < p.rows; row += step) {
+    float f[N][V], s[1] = {0.f};
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const Place<T> at(dim, l + G * i);
       if (!at.some) continue;
 #pragma unroll
-      for (int e = 0; e < V; ++e) s[0] += e < at.skip ? 0.f : f[i][e];
+      for (int e = 0; e < V; ++e) {
+        f[i][e] = (float)x[i].v[e];
+        s[0] += e < at.skip ? 0.f : f[i][e];
+      }
     }
+    if (row + step < p.rows) read(row + step);  // while this one is summed
     row_sum<G>(s, &lds[0]);
     const float mean = s[0] * over;
     s[0] = 0.f;
@@ -181,11 +190,8 @@ __global__ __launch_bounds__(kBlock<G>) void norm_fwd_kernel(NormFwd p) {
     for (int i = 0; i < N; ++i) {
       const Place<T> at(dim, l + G * i);
       if (!at.some) continue;
-      float w[V], b[V];
-      load_param<T>(p.w, p.w32, dim, at, 1.f, w);
-      load_param<T>(p.b, p.w32, dim, at, 0.f, b);
 #pragma unroll
-      for (int e = 0; e < V; ++e) f[i][e] = f[i][e] * r * w[e] + b[e];
+      for (int e = 0; e < V; ++e) f[i][e] = f[i][e] * r * w[i][e] + b[i][e];
       store_at<T>((T*)p.y + row * p.dim, dim, at, f[i]);
     }
     if (p.mean && l == 0) {
@@ -272,22 +278,24 @@ __global__ __launch_bounds__(kBlock<G>) void norm_bwd_kernel(NormBwd p) {
   float* out = p.partial + 2 * (int64_t)blockIdx.x * p.dim;
   if constexpr (R > 1) {
     // in the order of the groups, through LDS
-    __shared__ float sums[R][2][V * G];
-    static_assert(N == 1, "rows of one vector a lane share a block");
+    __shared__ float sums[R][V * G];
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      sums[group][0][e * G + l] = dw[0][e];
-      sums[group][1][e * G + l] = db[0][e];
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < 2 * V * G; i += kBlock<G>) {
-      const int which = i / (V * G), c = i % (V * G), j = c % G, e = c / G;
-      const Place<T> at(dim, j);
-      if (!at.some || at.from + e >= dim) continue;
-      float v = 0.f;
+    for (int k = 0; k < 2 * N; ++k) {
+      const int i = k % N, which = k / N;
+      __syncthreads();
 #pragma unroll
-      for (int k = 0; k < R; ++k) v += sums[k][which][c];
-      out[which * p.dim + at.from + e] = v;
+      for (int e = 0; e < V; ++e)
+        sums[group][e * G + l] = which ? db[i][e] : dw[i][e];
+      __syncthreads();
+      for (int c = threadIdx.x; c < V * G; c += kBlock<G>) {
+        const Place<T> at(dim, c % G + G * i);
+        const int e = c / G;
+        if (!at.some || at.from + e >= dim) continue;
+        float v = 0.f;
+#pragma unroll
+        for (int q = 0; q < R; ++q) v += sums[q][c];
+        out[which * p.dim + at.from + e] = v;
+      }
     }
   } else {
 #pragma unroll
@@ -381,24 +389,26 @@ __global__ __launch_bounds__(256) void norm_long_dw_kernel(NormBwd a) {
   a.partial[(2 * (int64_t)blockIdx.y + 1) * a.dim + i] = db;
 }
 
-// ---- dw and db from the blocks' shares: 32 columns a block, its 8 lanes a
-// column take every 8th share, then are added in their order
+// ---- dw and db from the blocks' shares: 32 columns a block, its 32 lanes a
+// column take every 32nd share, then are added in their order
+constexpr int kSumLanes = 32;
+
 template <typename W>
-__global__ __launch_bounds__(256) void norm_sum_kernel(NormSum a) {
-  __shared__ float lds[8][32];
+__global__ __launch_bounds__(32 * kSumLanes) void norm_sum_kernel(NormSum a) {
+  __shared__ float lds[kSumLanes][32];
   const int lane = threadIdx.x % 32, part = threadIdx.x / 32;
   const int64_t c = (int64_t)blockIdx.x * 32 + lane;  // of 2 D
   float v = 0.f;
   if (c < 2 * a.dim) {
 #pragma unroll 8
-    for (int k = part; k < a.parts; k += 8)
+    for (int k = part; k < a.parts; k += kSumLanes)
       v += a.partial[2 * k * a.dim + c];
   }
   lds[part][lane] = v;
   __syncthreads();
   if (part || c >= 2 * a.dim) return;
 #pragma unroll
-  for (int k = 1; k < 8; ++k) v += lds[k][lane];
+  for (int k = 1; k < kSumLanes; ++k) v += lds[k][lane];
   if (c < a.dim) {
     if (a.dw) ((W*)a.dw)[c] = (W)v;
   } else {
@@ -416,30 +426,31 @@ struct Shape {
 Shape shape_of(int64_t dim, int bytes) {
   const int64_t n = (dim * bytes + 15) / 16;  // vectors
   if (n <= 8) return {8, 1};
-  if (n <= 16) return {16, 1};
-  if (n <= 32) return {32, 1};
-  if (n <= 64) return {64, 1};
-  if (n <= 128) return {128, 1};
-  if (n <= 256) return {256, 1};
-  if (n <= 512) return {512, 1};
-  if (n <= 1024) return {1024, 1};
-  if (n <= 2048) return {1024, 2};
+  for (int G = 8; G <= 1024; G *= 2)
+    if (n <= 2 * G) return {G, 2};
   return {0, 0};
 }
 
 int parts_of(int64_t rows, int64_t dim, int bytes) {
   const Shape s = shape_of(dim, bytes);
-  const int64_t at_once = s.G == 0 ? 32 : s.G <= kWave ? 256 / s.G : 1;
-  const int64_t most = s.G == 0 ? 128 : s.G <= 256 ? 1024 : 256 * 1024 / s.G;
+  const int64_t at_once = s.G == 0 ? 32 : s.G <= kWave ? 512 / s.G : 1;
+  const int64_t most = s.G == 0     ? 128
+                       : s.G <= kWave ? 512
+                       : s.G < 256    ? 1024
+                       : s.G < 1024   ? 512
+                                      : 256;
   const int64_t p = (rows + at_once - 1) / at_once;
   return (int)(p < 1 ? 1 : p < most ? p : most);
 }
 
+constexpr int64_t kFwdLanes = 256 * 2048;  // of the forward pass, at most
+
 template <typename T, int G, int N>
 hipError_t fwd_with(const NormFwd& p, hipStream_t s) {
   constexpr int64_t R = kBlock<G> / G;
-  const int64_t grid = (p.rows + R - 1) / R;
-  return launch(norm_fwd_kernel<T, G, N>, dim3(grid < kGrid ? grid : kGrid),
+  const int64_t want = (p.rows + R - 1) / R;
+  const int64_t most = kFwdLanes / kBlock<G>;  // each walks rows from there on
+  return launch(norm_fwd_kernel<T, G, N>, dim3(want < most ? want : most),
                 dim3(kBlock<G>), 0, s, p);
 }
 
@@ -449,13 +460,13 @@ hipError_t fwd(const NormFwd& p, hipStream_t s) {
   const Shape h = shape_of(p.dim, sizeof(T));
   switch (h.G * 8 + h.N) {
     case 8 * 8 + 1: return fwd_with<T, 8, 1>(p, s);
-    case 16 * 8 + 1: return fwd_with<T, 16, 1>(p, s);
-    case 32 * 8 + 1: return fwd_with<T, 32, 1>(p, s);
-    case 64 * 8 + 1: return fwd_with<T, 64, 1>(p, s);
-    case 128 * 8 + 1: return fwd_with<T, 128, 1>(p, s);
-    case 256 * 8 + 1: return fwd_with<T, 256, 1>(p, s);
-    case 512 * 8 + 1: return fwd_with<T, 512, 1>(p, s);
-    case 1024 * 8 + 1: return fwd_with<T, 1024, 1>(p, s);
+    case 8 * 8 + 2: return fwd_with<T, 8, 2>(p, s);
+    case 16 * 8 + 2: return fwd_with<T, 16, 2>(p, s);
+    case 32 * 8 + 2: return fwd_with<T, 32, 2>(p, s);
+    case 64 * 8 + 2: return fwd_with<T, 64, 2>(p, s);
+    case 128 * 8 + 2: return fwd_with<T, 128, 2>(p, s);
+    case 256 * 8 + 2: return fwd_with<T, 256, 2>(p, s);
+    case 512 * 8 + 2: return fwd_with<T, 512, 2>(p, s);
     case 1024 * 8 + 2: return fwd_with<T, 1024, 2>(p, s);
   }
   return launch(norm_long_fwd_kernel<T>,
@@ -474,13 +485,13 @@ hipError_t bwd(const NormBwd& p, const NormSum& z, hipStream_t s) {
   hipError_t e = hipSuccess;
   switch (h.G * 8 + h.N) {
     case 8 * 8 + 1: e = bwd_with<T, 8, 1>(p, s); break;
-    case 16 * 8 + 1: e = bwd_with<T, 16, 1>(p, s); break;
-    case 32 * 8 + 1: e = bwd_with<T, 32, 1>(p, s); break;
-    case 64 * 8 + 1: e = bwd_with<T, 64, 1>(p, s); break;
-    case 128 * 8 + 1: e = bwd_with<T, 128, 1>(p, s); break;
-    case 256 * 8 + 1: e = bwd_with<T, 256, 1>(p, s); break;
-    case 512 * 8 + 1: e = bwd_with<T, 512, 1>(p, s); break;
-    case 1024 * 8 + 1: e = bwd_with<T, 1024, 1>(p, s); break;
+    case 8 * 8 + 2: e = bwd_with<T, 8, 2>(p, s); break;
+    case 16 * 8 + 2: e = bwd_with<T, 16, 2>(p, s); break;
+    case 32 * 8 + 2: e = bwd_with<T, 32, 2>(p, s); break;
+    case 64 * 8 + 2: e = bwd_with<T, 64, 2>(p, s); break;
+    case 128 * 8 + 2: e = bwd_with<T, 128, 2>(p, s); break;
+    case 256 * 8 + 2: e = bwd_with<T, 256, 2>(p, s); break;
+    case 512 * 8 + 2: e = bwd_with<T, 512, 2>(p, s); break;
     case 1024 * 8 + 2: e = bwd_with<T, 1024, 2>(p, s); break;
     default:
       if (p.dx && p.rows > 0)
@@ -492,8 +503,8 @@ hipError_t bwd(const NormBwd& p, const NormSum& z, hipStream_t s) {
   }
   if (e != hipSuccess || !p.partial) return e;
   const dim3 grid((2 * p.dim + 31) / 32);
-  if (p.w32) return launch(norm_sum_kernel<float>, grid, dim3(256), 0, s, z);
-  return launch(norm_sum_kernel<T>, grid, dim3(256), 0, s, z);
+  if (p.w32) return launch(norm_sum_kernel<float>, grid, dim3(32 * kSumLanes), 0, s, z);
+  return launch(norm_sum_kernel<T>, grid, dim3(32 * kSumLanes), 0, s, z);
 }
 
 }  // namespace
