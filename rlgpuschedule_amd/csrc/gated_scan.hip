@@ -22,7 +22,7 @@
 namespace {
 using namespace seq;
 
-constexpr int kKeep = 16;  // steps from one kept state to the next
+constexpr int kKeep = 8;  // steps from one kept state to the next
 
 // A sequence's columns as lanes: n lanes an environment, the last of which
 // begins early enough to end with it and computes shared columns twice, to
@@ -97,15 +97,15 @@ __device__ __forceinline__ void gates(float g, float& z, float& a) {
   const float q = e * r;
   z = g >= 0.f ? r : q;
   a = g >= 0.f ? q : r;
-  if (g != g) z = a = g;
 }
 
 // A state's way through some steps: c_end = A c_start + B, or B alone (A
 // below zero) where an episode ended within them.
 struct Way {
   float A = 1.f, B = 0.f;
+  template <bool DONE>
   __device__ __forceinline__ void step(float a, float b) {
-    A = A < 0.f ? A : A * a;
+    A = DONE && A < 0.f ? A : A * a;
     B = a * B + b;
   }
   __device__ __forceinline__ void end() {
@@ -119,11 +119,32 @@ struct Way {
 };
 
 // ---- forward
-// The k-th step from t, or the last before `end`: what is behind it is read
-// there and not used. FULL: there is nothing behind it.
-template <bool FULL>
-__device__ __forceinline__ int64_t step_at(int64_t t, int k, int64_t end) {
-  return FULL || t + k < end ? k : end - 1 - t;
+// N steps of a lane's columns from t on. FULL: all of them are before `end`;
+// else what is not is not read.
+template <bool FULL, typename T, int V, int N>
+__device__ __forceinline__ void read_steps(Vec<T, V> (&to)[N], const T* from,
+                                           int64_t stride_t, int64_t stride_e,
+                                           const Lane& l, int64_t t,
+                                           int64_t end) {
+  const T* at = here(from + t * stride_t, l, stride_e);
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    if (!FULL) to[k] = {};
+    if (FULL || t + k < end) to[k] = load<T, V>(at + k * stride_t);
+  }
+}
+
+// Which of N steps end an episode, a bit each.
+template <bool FULL, int N>
+__device__ __forceinline__ uint32_t ends_of(const uint8_t* done, int64_t E,
+                                            const Lane& l, int64_t t,
+                                            int64_t end) {
+  const uint8_t* at = done + t * E + l.e0 + l.e;
+  uint32_t ends = 0;
+#pragma unroll
+  for (int k = 0; k < N; ++k)
+    if (FULL || t + k < end) ends |= (uint32_t)(at[k * E] != 0) << k;
+  return ends;
 }
 
 // L steps of a lane's columns, and which of them end an episode.
@@ -132,28 +153,17 @@ struct Steps {
   Vec<T, V> gate[L], x[L];
   uint32_t ends;
 
-  template <bool FULL>
+  template <bool FULL, bool DONE>
   __device__ __forceinline__ void read(const ScanFwd& p, const Lane& l,
                                        int64_t t, int64_t end) {
-    const T* g = here((const T*)p.gate + t * p.gate_t, l, p.gate_e);
-    const T* v = here((const T*)p.x + t * p.x_t, l, p.x_e);
-#pragma unroll
-    for (int k = 0; k < L; ++k) {
-      const int64_t i = step_at<FULL>(t, k, end);
-      gate[k] = load<T, V>(g + i * p.gate_t);
-      x[k] = load<T, V>(v + i * p.x_t);
-    }
+    read_steps<FULL>(gate, (const T*)p.gate, p.gate_t, p.gate_e, l, t, end);
+    read_steps<FULL>(x, (const T*)p.x, p.x_t, p.x_e, l, t, end);
     ends = 0;
-    if (p.done) {
-      const uint8_t* d = p.done + t * p.c.E + l.e0 + l.e;
-#pragma unroll
-      for (int k = 0; k < L; ++k)
-        ends |= (uint32_t)(d[step_at<FULL>(t, k, end) * p.c.E] != 0) << k;
-    }
+    if constexpr (DONE) ends = ends_of<FULL, L>(p.done, p.c.E, l, t, end);
   }
 };
 
-template <bool FULL, typename T, int V, int L>
+template <bool FULL, bool DONE, typename T, int V, int L>
 __device__ __forceinline__ void walk(const ScanFwd& p, const Lane& l,
                                      const Steps<T, V, L>& s, int64_t t,
                                      int64_t end, float (&c)[V]) {
@@ -170,7 +180,7 @@ __device__ __forceinline__ void walk(const ScanFwd& p, const Lane& l,
       float z, a;
       gates((float)s.gate[k].v[v], z, a);
       h[v] = a * c[v] + z * (float)s.x[k].v[v];
-      c[v] = s.ends >> k & 1 ? 0.f : h[v];
+      c[v] = DONE && (s.ends >> k & 1) ? 0.f : h[v];
     }
     store<T, V>(out + k * EH, h);
   }
@@ -178,7 +188,7 @@ __device__ __forceinline__ void walk(const ScanFwd& p, const Lane& l,
 
 // kKeep is a multiple of L and a chunk one of kKeep, so states lie at the
 // first of L steps.
-template <typename T, int V, int L>
+template <typename T, int V, int L, bool DONE>
 __global__ __launch_bounds__(256) void scan_fwd_kernel(ScanFwd p) {
   static_assert(kKeep % L == 0, "states are kept between steps read at once");
   Lane l;
@@ -195,28 +205,28 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(ScanFwd p) {
   if (t + L <= end) {
     // the next steps are read while these are walked
     Steps<T, V, L> s, n;
-    s.template read<true>(p, l, t, end);
+    s.template read<true, DONE>(p, l, t, end);
     for (; t + 2 * L <= end; t += L) {
-      n.template read<true>(p, l, t + L, end);
-      walk<true>(p, l, s, t, end, c);
+      n.template read<true, DONE>(p, l, t + L, end);
+      walk<true, DONE>(p, l, s, t, end, c);
       s = n;
     }
-    walk<true>(p, l, s, t, end, c);
+    walk<true, DONE>(p, l, s, t, end, c);
     t += L;
   }
   if (t < end) {
     Steps<T, V, L> s;
-    s.template read<false>(p, l, t, end);
-    walk<false>(p, l, s, t, end, c);
+    s.template read<false, DONE>(p, l, t, end);
+    walk<false, DONE>(p, l, s, t, end, c);
   }
   if (end == p.T) store<float, V>(here(p.h_last, l, p.c.H), c);
 }
 
-template <bool FULL, typename T, int V, int L>
+template <bool FULL, bool DONE, typename T, int V, int L>
 __device__ __forceinline__ void way(const ScanFwd& p, const Lane& l, int64_t t,
                                     int64_t end, Way (&w)[V]) {
   Steps<T, V, L> s;
-  s.template read<FULL>(p, l, t, end);
+  s.template read<FULL, DONE>(p, l, t, end);
 #pragma unroll
   for (int k = 0; k < L; ++k) {
     if (!FULL && t + k >= end) continue;
@@ -224,8 +234,8 @@ __device__ __forceinline__ void way(const ScanFwd& p, const Lane& l, int64_t t,
     for (int v = 0; v < V; ++v) {
       float z, a;
       gates((float)s.gate[k].v[v], z, a);
-      w[v].step(a, z * (float)s.x[k].v[v]);
-      if (s.ends >> k & 1) w[v].end();
+      w[v].template step<DONE>(a, z * (float)s.x[k].v[v]);
+      if (DONE && (s.ends >> k & 1)) w[v].end();
     }
   }
 }
@@ -241,7 +251,7 @@ __device__ __forceinline__ void keep_way(const Cols& c, const Lane& l,
   store<float, V>(here(ways + (2 * k + 1) * EH, l, c.H), B);
 }
 
-template <typename T, int V>
+template <typename T, int V, bool DONE>
 __global__ __launch_bounds__(256) void scan_fwd_way_kernel(ScanFwd p,
                                                            float* ways) {
   constexpr int L = kKeep;
@@ -250,8 +260,8 @@ __global__ __launch_bounds__(256) void scan_fwd_way_kernel(ScanFwd p,
   int64_t t = blockIdx.y * p.chunk;
   const int64_t end = t + p.chunk < p.T ? t + p.chunk : p.T;
   Way w[V];
-  for (; t + L <= end; t += L) way<true, T, V, L>(p, l, t, end, w);
-  if (t < end) way<false, T, V, L>(p, l, t, end, w);
+  for (; t + L <= end; t += L) way<true, DONE, T, V, L>(p, l, t, end, w);
+  if (t < end) way<false, DONE, T, V, L>(p, l, t, end, w);
   keep_way<V>(p.c, l, w, ways);
 }
 
@@ -319,36 +329,25 @@ struct Back {
   Vec<T, V> gate[kKeep], dhs[kKeep];
   uint32_t ends = 0;
 
-  template <bool FULL>
+  template <bool FULL, bool DONE>
   __device__ __forceinline__ void read(const ScanBwd& p, const Lane& l,
                                        int64_t t, int64_t end) {
-    const T* g = here((const T*)p.gate + t * p.gate_t, l, p.gate_e);
-#pragma unroll
-    for (int k = 0; k < kKeep; ++k)
-      gate[k] = load<T, V>(g + step_at<FULL>(t, k, end) * p.gate_t);
+    read_steps<FULL>(gate, (const T*)p.gate, p.gate_t, p.gate_e, l, t, end);
     if (p.dhs) {
-      const T* h = here((const T*)p.dhs + t * p.dhs_t, l, p.dhs_e);
-#pragma unroll
-      for (int k = 0; k < kKeep; ++k)
-        dhs[k] = load<T, V>(h + step_at<FULL>(t, k, end) * p.dhs_t);
+      read_steps<FULL>(dhs, (const T*)p.dhs, p.dhs_t, p.dhs_e, l, t, end);
     } else {
 #pragma unroll
       for (int k = 0; k < kKeep; ++k) dhs[k] = {};
     }
-    if (p.done) {
-      const uint8_t* d = p.done + t * p.c.E + l.e0 + l.e;
-#pragma unroll
-      for (int k = 0; k < kKeep; ++k)
-        ends |= (uint32_t)(d[step_at<FULL>(t, k, end) * p.c.E] != 0) << k;
-    }
+    if constexpr (DONE) ends = ends_of<FULL, kKeep>(p.done, p.c.E, l, t, end);
   }
 };
 
-template <bool FULL, typename T, int V>
+template <bool FULL, bool DONE, typename T, int V>
 __device__ __forceinline__ void way_back(const ScanBwd& p, const Lane& l,
                                          int64_t t, int64_t end, Way (&w)[V]) {
   Back<T, V> s;
-  s.template read<FULL>(p, l, t, end);
+  s.template read<FULL, DONE>(p, l, t, end);
 #pragma unroll
   for (int k = kKeep - 1; k >= 0; --k) {
     if (!FULL && t + k >= end) continue;
@@ -356,13 +355,13 @@ __device__ __forceinline__ void way_back(const ScanBwd& p, const Lane& l,
     for (int v = 0; v < V; ++v) {
       float z, a;
       gates((float)s.gate[k].v[v], z, a);
-      if (s.ends >> k & 1) w[v].end();
-      w[v].step(a, a * (float)s.dhs[k].v[v]);
+      if (DONE && (s.ends >> k & 1)) w[v].end();
+      w[v].template step<DONE>(a, a * (float)s.dhs[k].v[v]);
     }
   }
 }
 
-template <typename T, int V>
+template <typename T, int V, bool DONE>
 __global__ __launch_bounds__(256) void scan_bwd_way_kernel(ScanBwd p,
                                                            float* ways) {
   Lane l;
@@ -371,13 +370,31 @@ __global__ __launch_bounds__(256) void scan_bwd_way_kernel(ScanBwd p,
   const int64_t end = t0 + p.chunk < p.T ? t0 + p.chunk : p.T;
   int64_t t = t0 + (end - t0) / kKeep * kKeep;
   Way w[V];
-  if (t < end) way_back<false, T, V>(p, l, t, end, w);
+  if (t < end) way_back<false, DONE, T, V>(p, l, t, end, w);
   for (t -= kKeep; t >= t0; t -= kKeep)
-    way_back<true, T, V>(p, l, t, end, w);
+    way_back<true, DONE, T, V>(p, l, t, end, w);
   keep_way<V>(p.c, l, w, ways);
 }
 
-template <bool FULL, typename T, int V>
+// The compiler takes the values as new ones.
+template <typename T, int V>
+__device__ __forceinline__ void forget(Vec<T, V>& x) {
+  if constexpr (sizeof(x) == 2) {
+    uint16_t w;
+    __builtin_memcpy(&w, &x, 2);
+    asm volatile("" : "+v"(w));
+    __builtin_memcpy(&x, &w, 2);
+  } else {
+    uint32_t w[sizeof(x) / 4];
+    __builtin_memcpy(w, &x, sizeof(x));
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(x) / 4); ++i)
+      asm volatile("" : "+v"(w[i]));
+    __builtin_memcpy(&x, w, sizeof(x));
+  }
+}
+
+template <bool FULL, bool DONE, typename T, int V>
 __device__ __forceinline__ void walk_back(const ScanBwd& p, const Lane& l,
                                           int64_t t, int64_t end,
                                           float (&carry)[V]) {
@@ -386,11 +403,8 @@ __device__ __forceinline__ void walk_back(const ScanBwd& p, const Lane& l,
   Vec<T, V> x[kKeep];
   float c[V], diff[kKeep][V];  // x - c
   load<float, V>(here(p.states + t / kKeep * EH, l, p.c.H), c);
-  const T* v0 = here((const T*)p.x + t * p.x_t, l, p.x_e);
-#pragma unroll
-  for (int k = 0; k < kKeep; ++k)
-    x[k] = load<T, V>(v0 + step_at<FULL>(t, k, end) * p.x_t);
-  s.template read<FULL>(p, l, t, end);
+  read_steps<FULL>(x, (const T*)p.x, p.x_t, p.x_e, l, t, end);
+  s.template read<FULL, DONE>(p, l, t, end);
 #pragma unroll
   for (int k = 0; k < kKeep; ++k) {
     if (!FULL && t + k >= end) continue;
@@ -400,9 +414,13 @@ __device__ __forceinline__ void walk_back(const ScanBwd& p, const Lane& l,
       gates((float)s.gate[k].v[v], z, a);
       const float xv = (float)x[k].v[v];
       diff[k][v] = xv - c[v];
-      c[v] = s.ends >> k & 1 ? 0.f : a * c[v] + z * xv;
+      c[v] = DONE && (s.ends >> k & 1) ? 0.f : a * c[v] + z * xv;
     }
   }
+  // The gates are computed again: kept, they would take the registers of half
+  // the waves.
+#pragma unroll
+  for (int k = 0; k < kKeep; ++k) forget(s.gate[k]);
   T* out_x = here((T*)p.dx + t * EH, l, p.c.H);
   T* out_g = here((T*)p.dgate + t * EH, l, p.c.H);
 #pragma unroll
@@ -413,8 +431,8 @@ __device__ __forceinline__ void walk_back(const ScanBwd& p, const Lane& l,
     for (int v = 0; v < V; ++v) {
       float z, a;
       gates((float)s.gate[k].v[v], z, a);
-      const float D =
-          (s.ends >> k & 1 ? 0.f : carry[v]) + (float)s.dhs[k].v[v];
+      const bool ends = DONE && (s.ends >> k & 1);
+      const float D = (ends ? 0.f : carry[v]) + (float)s.dhs[k].v[v];
       dx[v] = z * D;
       dg[v] = D * diff[k][v] * (z * a);
       carry[v] = a * D;
@@ -424,7 +442,7 @@ __device__ __forceinline__ void walk_back(const ScanBwd& p, const Lane& l,
   }
 }
 
-template <typename T, int V>
+template <typename T, int V, bool DONE>
 __global__ __launch_bounds__(256) void scan_bwd_kernel(ScanBwd p) {
   Lane l;
   if (!lane_of<V>(p.c, l)) return;
@@ -438,9 +456,9 @@ __global__ __launch_bounds__(256) void scan_bwd_kernel(ScanBwd p) {
     load<float, V>(here(p.dh_last, l, p.c.H), carry);
   }
   int64_t t = t0 + (end - t0) / kKeep * kKeep;
-  if (t < end) walk_back<false, T, V>(p, l, t, end, carry);
+  if (t < end) walk_back<false, DONE, T, V>(p, l, t, end, carry);
   for (t -= kKeep; t >= t0; t -= kKeep)
-    walk_back<true, T, V>(p, l, t, end, carry);
+    walk_back<true, DONE, T, V>(p, l, t, end, carry);
   if (t0 == 0 && p.dh0) store<float, V>(here(p.dh0, l, p.c.H), carry);
 }
 
@@ -496,19 +514,25 @@ struct Plan {
   int64_t n, chunk, chunks;
 };
 
-constexpr int64_t kWaves = 2048;  // as many keep the memory busy
+constexpr int64_t kWaves = 4096;  // as many keep the memory busy
 constexpr int64_t kShort = 128;   // steps that one lane walks in any case
 
-Plan plan(int64_t T, int64_t E, int64_t H) {
+// Lanes take 8 bytes of columns, or fewer where that leaves too few waves.
+Plan plan(int64_t T, int64_t E, int64_t H, int bytes) {
   Plan p;
-  p.V = H < 2 ? 1 : 2;
-  p.n = (H + p.V - 1) / p.V;
-  const int64_t waves = (E * p.n + kWave - 1) / kWave;
+  int64_t waves = 0;
+  for (p.V = 8 / bytes; p.V >= 1; p.V /= 2) {
+    if (p.V > H) continue;
+    p.n = (H + p.V - 1) / p.V;
+    waves = (E * p.n + kWave - 1) / kWave;
+    const int64_t cuts = T > kShort ? T / 64 : 1;
+    if (p.V == 1 || waves * cuts >= kWaves / 4) break;
+  }
   p.chunk = T;
   p.chunks = 1;
-  if (T > kShort && waves < kWaves) {
-    int64_t want = 2 * kWaves / waves;  // chunks
-    const int64_t most = (T + 63) / 64;
+  if (T > kShort && waves < kWaves / 2) {
+    int64_t want = kWaves / waves;  // chunks
+    const int64_t most = (T + 15) / 16;
     want = want < most ? want : most;
     want = want < 32768 ? want : 32768;
     if (want > 1) {
@@ -532,62 +556,81 @@ hipError_t join(const float* ways, const float* first, float* carry,
                 0, s, j);
 }
 
-template <typename T, int V, int L>
+template <typename T, int V, bool DONE>
 hipError_t fwd_with(const ScanFwd& p, const Plan& q, float* ways,
                     hipStream_t s) {
   const int64_t EH = p.c.E * p.c.H;
   const dim3 grid((p.c.E * p.c.n + 255) / 256, q.chunks);
   if (q.chunks > 1) {
-    hipError_t e = launch(scan_fwd_way_kernel<T, V>, grid, dim3(256), 0, s,
+    hipError_t e = launch(scan_fwd_way_kernel<T, V, DONE>, grid, dim3(256), 0, s,
                           p, ways);
     if (e == hipSuccess) e = join(ways, p.h0, p.carry, q, EH, false, s);
     if (e != hipSuccess) return e;
   }
-  return launch(scan_fwd_kernel<T, V, L>, grid, dim3(256), 0, s, p);
+  return launch(scan_fwd_kernel<T, V, kKeep, DONE>, grid, dim3(256), 0, s, p);
 }
 
 template <typename T>
 hipError_t fwd(ScanFwd p, float* scratch, hipStream_t s) {
   if (p.c.E * p.c.H == 0) return hipSuccess;
-  const Plan q = plan(p.T, p.c.E, p.c.H);
+  const Plan q = plan(p.T, p.c.E, p.c.H, sizeof(T));
   p.c.n = q.n;
   p.chunk = q.chunk;
   p.carry = carry_of(q, scratch, p.c.E * p.c.H);
-  if (q.V == 2) return fwd_with<T, 2, 8>(p, q, scratch, s);
-  return fwd_with<T, 1, 8>(p, q, scratch, s);
+  switch (q.V * 2 + (p.done != nullptr)) {
+    case 2: return fwd_with<T, 1, false>(p, q, scratch, s);
+    case 3: return fwd_with<T, 1, true>(p, q, scratch, s);
+    case 4: return fwd_with<T, 2, false>(p, q, scratch, s);
+    case 5: return fwd_with<T, 2, true>(p, q, scratch, s);
+  }
+  if constexpr (sizeof(T) == 2) {
+    if (p.done) return fwd_with<T, 4, true>(p, q, scratch, s);
+    return fwd_with<T, 4, false>(p, q, scratch, s);
+  }
+  return hipErrorInvalidValue;
 }
 
-template <typename T, int V>
+template <typename T, int V, bool DONE>
 hipError_t bwd_with(const ScanBwd& p, const Plan& q, float* ways,
                     hipStream_t s) {
   const int64_t EH = p.c.E * p.c.H;
   const dim3 grid((p.c.E * p.c.n + 255) / 256, q.chunks);
   if (q.chunks > 1) {
     hipError_t e =
-        launch(scan_bwd_way_kernel<T, V>, grid, dim3(256), 0, s, p, ways);
+        launch(scan_bwd_way_kernel<T, V, DONE>, grid, dim3(256), 0, s, p, ways);
     if (e == hipSuccess) e = join(ways, p.dh_last, p.carry, q, EH, true, s);
     if (e != hipSuccess) return e;
   }
-  return launch(scan_bwd_kernel<T, V>, grid, dim3(256), 0, s, p);
+  return launch(scan_bwd_kernel<T, V, DONE>, grid, dim3(256), 0, s, p);
 }
 
 template <typename T>
 hipError_t bwd(ScanBwd p, float* scratch, hipStream_t s) {
   if (p.c.E * p.c.H == 0) return hipSuccess;
-  const Plan q = plan(p.T, p.c.E, p.c.H);
+  const Plan q = plan(p.T, p.c.E, p.c.H, sizeof(T));
   p.c.n = q.n;
   p.chunk = q.chunk;
   p.carry = carry_of(q, scratch, p.c.E * p.c.H);
-  if (q.V == 2) return bwd_with<T, 2>(p, q, scratch, s);
-  return bwd_with<T, 1>(p, q, scratch, s);
+  switch (q.V * 2 + (p.done != nullptr)) {
+    case 2: return bwd_with<T, 1, false>(p, q, scratch, s);
+    case 3: return bwd_with<T, 1, true>(p, q, scratch, s);
+    case 4: return bwd_with<T, 2, false>(p, q, scratch, s);
+    case 5: return bwd_with<T, 2, true>(p, q, scratch, s);
+  }
+  if constexpr (sizeof(T) == 2) {
+    if (p.done) return bwd_with<T, 4, true>(p, q, scratch, s);
+    return bwd_with<T, 4, false>(p, q, scratch, s);
+  }
+  return hipErrorInvalidValue;
 }
 
 }  // namespace
 
 // Floats of scratch that the forward and the backward call each need.
-extern "C" int64_t rlsched_scan_scratch(int64_t T, int64_t E, int64_t H) {
+extern "C" int64_t rlsched_scan_scratch(int64_t T, int64_t E, int64_t H,
+                                        int type) {
   if (E * H == 0) return 0;
-  const Plan q = plan(T, E, H);
+  const Plan q = plan(T, E, H, type == F32 ? 4 : 2);
   return q.chunks > 1 ? 3 * q.chunks * E * H : 0;
 }
 

@@ -328,8 +328,8 @@ int check_scan(const Tensor& gate, const Tensor& x, const MaybeTensor& h,
               " and ", x.sizes(), " ", x.scalar_type());
   const int code = type_code(x, "x");
   const int64_t E = x.size(-2), H = x.size(-1);
-  VALUE_CHECK(E == 0 || H < (1ll << 31) / E, E, " x ", H,
-              " columns: fewer than 2**31 are supported");
+  VALUE_CHECK(E == 0 || H < (1ll << 28) / E, E, " x ", H,
+              " columns: fewer than 2**28 are supported");
   if (h) {
     VALUE_CHECK(h->dim() == 2 && h->size(0) == E && h->size(1) == H &&
                     h->scalar_type() == at::kFloat,
@@ -360,7 +360,8 @@ std::tuple<Tensor, Tensor, Tensor> scan_fwd(const Tensor& gate_,
   Tensor h_last = f32(x_, {E, H}), states;
   if (keep) states = f32(x_, {rlsched_scan_states(T), E, H});
   Tensor scratch;
-  if (const int64_t n = rlsched_scan_scratch(T, E, H)) scratch = f32(x_, {n});
+  if (const int64_t n = rlsched_scan_scratch(T, E, H, type))
+    scratch = f32(x_, {n});
   const Tensor gate = reachable(gate_), x = reachable(x_);
   const MaybeTensor h0 = packed(h0_), done = packed(done_);
   const Place at(x);
@@ -399,7 +400,8 @@ std::tuple<Tensor, Tensor, Tensor> scan_bwd(
   Tensor dx = at::empty({T, E, H}, like_x), dh0;
   if (need_dh0) dh0 = f32(x_, {E, H});
   Tensor scratch;
-  if (const int64_t n = rlsched_scan_scratch(T, E, H)) scratch = f32(x_, {n});
+  if (const int64_t n = rlsched_scan_scratch(T, E, H, type))
+    scratch = f32(x_, {n});
   const Tensor gate = reachable(gate_), x = reachable(x_);
   MaybeTensor dhs;
   if (dhs_) dhs = reachable(*dhs_);

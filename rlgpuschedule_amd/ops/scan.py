@@ -24,7 +24,7 @@ def gated_scan_fwd(gate: torch.Tensor, x: torch.Tensor,
                    keep_states: bool = True):
     """gate, x [T, E, H] on a GPU (float32, bfloat16 or float16; any strides
     of time and environment, such as the halves of one projection; fewer than
-    2**31 columns E H), h0 [E, H] f32 or None (zeros), done [T, E] u8/bool or
+    2**28 columns E H), h0 [E, H] f32 or None (zeros), done [T, E] u8/bool or
     None. Returns (hs [T, E, H] of x's type, h_last [E, H] f32, states):
     states is what gated_scan_bwd needs (None without keep_states)."""
     return ext().gated_scan_fwd(gate, x, h0, done, keep_states)
