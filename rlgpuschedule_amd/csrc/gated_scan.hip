@@ -240,13 +240,19 @@ __device__ __forceinline__ void way(const ScanFwd& p, const Lane& l, int64_t t,
   }
 }
 
+// The chunks' effects are found from the last to the first, so that the
+// kernel that walks them begins with what was read last and is still cached.
+__device__ __forceinline__ int64_t from_last() {
+  return gridDim.y - 1 - blockIdx.y;
+}
+
 template <int V>
 __device__ __forceinline__ void keep_way(const Cols& c, const Lane& l,
                                          const Way (&w)[V], float* ways) {
   float A[V], B[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) A[v] = w[v].A, B[v] = w[v].B;
-  const int64_t EH = c.E * c.H, k = blockIdx.y;
+  const int64_t EH = c.E * c.H, k = from_last();
   store<float, V>(here(ways + 2 * k * EH, l, c.H), A);
   store<float, V>(here(ways + (2 * k + 1) * EH, l, c.H), B);
 }
@@ -257,7 +263,7 @@ __global__ __launch_bounds__(256) void scan_fwd_way_kernel(ScanFwd p,
   constexpr int L = kKeep;
   Lane l;
   if (!lane_of<V>(p.c, l)) return;
-  int64_t t = blockIdx.y * p.chunk;
+  int64_t t = from_last() * p.chunk;
   const int64_t end = t + p.chunk < p.T ? t + p.chunk : p.T;
   Way w[V];
   for (; t + L <= end; t += L) way<true, DONE, T, V, L>(p, l, t, end, w);
@@ -267,7 +273,7 @@ __global__ __launch_bounds__(256) void scan_fwd_way_kernel(ScanFwd p,
 
 // ---- from chunk to chunk, in either direction: 64 columns a block, its 16
 // waves one after the other in time, kJoin chunks each
-constexpr int kJoin = 8;
+constexpr int kJoin = 16;
 
 struct Join {
   const float* ways;   // [chunks, 2, EH]
@@ -366,7 +372,7 @@ __global__ __launch_bounds__(256) void scan_bwd_way_kernel(ScanBwd p,
                                                            float* ways) {
   Lane l;
   if (!lane_of<V>(p.c, l)) return;
-  const int64_t t0 = blockIdx.y * p.chunk;
+  const int64_t t0 = from_last() * p.chunk;
   const int64_t end = t0 + p.chunk < p.T ? t0 + p.chunk : p.T;
   int64_t t = t0 + (end - t0) / kKeep * kKeep;
   Way w[V];
@@ -394,17 +400,30 @@ __device__ __forceinline__ void forget(Vec<T, V>& x) {
   }
 }
 
-template <bool FULL, bool DONE, typename T, int V>
-__device__ __forceinline__ void walk_back(const ScanBwd& p, const Lane& l,
-                                          int64_t t, int64_t end,
-                                          float (&carry)[V]) {
-  const int64_t EH = p.c.E * p.c.H;
+// What kKeep steps of a lane's columns are walked back with.
+template <typename T, int V>
+struct Sheet {
   Back<T, V> s;
   Vec<T, V> x[kKeep];
-  float c[V], diff[kKeep][V];  // x - c
-  load<float, V>(here(p.states + t / kKeep * EH, l, p.c.H), c);
-  read_steps<FULL>(x, (const T*)p.x, p.x_t, p.x_e, l, t, end);
-  s.template read<FULL, DONE>(p, l, t, end);
+  float c[V];  // before the first
+
+  template <bool FULL, bool DONE>
+  __device__ __forceinline__ void read(const ScanBwd& p, const Lane& l,
+                                       int64_t t, int64_t end) {
+    load<float, V>(here(p.states + t / kKeep * p.c.E * p.c.H, l, p.c.H), c);
+    read_steps<FULL>(x, (const T*)p.x, p.x_t, p.x_e, l, t, end);
+    s.ends = 0;
+    s.template read<FULL, DONE>(p, l, t, end);
+  }
+};
+
+template <bool FULL, bool DONE, typename T, int V>
+__device__ __forceinline__ void walk_back(const ScanBwd& p, const Lane& l,
+                                          Sheet<T, V>& now, int64_t t,
+                                          int64_t end, float (&carry)[V]) {
+  const int64_t EH = p.c.E * p.c.H;
+  Back<T, V>& s = now.s;
+  float diff[kKeep][V];  // x - c
 #pragma unroll
   for (int k = 0; k < kKeep; ++k) {
     if (!FULL && t + k >= end) continue;
@@ -412,9 +431,9 @@ __device__ __forceinline__ void walk_back(const ScanBwd& p, const Lane& l,
     for (int v = 0; v < V; ++v) {
       float z, a;
       gates((float)s.gate[k].v[v], z, a);
-      const float xv = (float)x[k].v[v];
-      diff[k][v] = xv - c[v];
-      c[v] = DONE && (s.ends >> k & 1) ? 0.f : a * c[v] + z * xv;
+      const float xv = (float)now.x[k].v[v];
+      diff[k][v] = xv - now.c[v];
+      now.c[v] = DONE && (s.ends >> k & 1) ? 0.f : a * now.c[v] + z * xv;
     }
   }
   // The gates are computed again: kept, they would take the registers of half
@@ -456,9 +475,27 @@ __global__ __launch_bounds__(256) void scan_bwd_kernel(ScanBwd p) {
     load<float, V>(here(p.dh_last, l, p.c.H), carry);
   }
   int64_t t = t0 + (end - t0) / kKeep * kKeep;
-  if (t < end) walk_back<false, DONE, T, V>(p, l, t, end, carry);
-  for (t -= kKeep; t >= t0; t -= kKeep)
-    walk_back<true, DONE, T, V>(p, l, t, end, carry);
+  Sheet<T, V> now;
+  if (t < end) {
+    now.template read<false, DONE>(p, l, t, end);
+    walk_back<false, DONE>(p, l, now, t, end, carry);
+  }
+  t -= kKeep;
+  if constexpr (sizeof(T) * V < 8) {
+    // few waves: the steps before are read while these are walked
+    Sheet<T, V> next;
+    if (t >= t0) now.template read<true, DONE>(p, l, t, end);
+    for (; t >= t0; t -= kKeep) {
+      if (t > t0) next.template read<true, DONE>(p, l, t - kKeep, end);
+      walk_back<true, DONE>(p, l, now, t, end, carry);
+      now = next;
+    }
+  } else {
+    for (; t >= t0; t -= kKeep) {
+      now.template read<true, DONE>(p, l, t, end);
+      walk_back<true, DONE>(p, l, now, t, end, carry);
+    }
+  }
   if (t0 == 0 && p.dh0) store<float, V>(here(p.dh0, l, p.c.H), carry);
 }
 
