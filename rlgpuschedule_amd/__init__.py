@@ -7,7 +7,8 @@ and IMPALA-style async actor/learner, with data parallelism over RCCL/xGMI.
 
 Public API (lazy imports; heavy deps load on first use):
     EnvSpec, cluster16/64/256/1024, ClusterSchedEnv, CpuVectorEnv,
-    HipVectorEnv, MLPPolicy, GRUPolicy, TrainConfig, CONFIGS, train,
+    HipVectorEnv, MLPPolicy, GRUPolicy, LinearRecurrentPolicy, TrainConfig,
+    CONFIGS, train,
     JobTrace, philly_like, poisson,
     layer_norm, gated_scan, gated_scan_step, action_logprobs
 """
@@ -24,6 +25,7 @@ _EXPORTS = {
     "HipVectorEnv": "rlgpuschedule_amd.env.hip_env",
     "MLPPolicy": "rlgpuschedule_amd.models.policy",
     "GRUPolicy": "rlgpuschedule_amd.models.policy",
+    "LinearRecurrentPolicy": "rlgpuschedule_amd.models.policy",
     "TrainConfig": "rlgpuschedule_amd.trainer",
     "CONFIGS": "rlgpuschedule_amd.trainer",
     "train": "rlgpuschedule_amd.trainer",

@@ -13,6 +13,7 @@ import torch.nn.functional as F
 
 from ..models.policy import evaluate_actions
 from ..ops.gae_ref import gae_advantages
+from ..ops.logprob import action_logprobs
 from .rollout import RolloutBuffer
 
 
@@ -24,6 +25,27 @@ def compute_gae(buf: RolloutBuffer, gamma: float, lam: float):
                         gamma, lam)
     return gae_advantages(buf.reward, buf.value, buf.done, buf.last_value,
                           gamma, lam)
+
+
+def replay_sequence(policy, obs, mask, actions, h0, done):
+    """Log probabilities, entropies and values [T, E] of a recurrent policy
+    along stored sequences, from h0 and with its state reset at the stored
+    done flags. Policies with forward_sequence replay all of it at once,
+    others step by step."""
+    if hasattr(policy, "forward_sequence"):
+        logits, value, _ = policy.forward_sequence(obs, h0, done)
+        r = action_logprobs(logits, actions, mask)
+        return r.logp, r.entropy, value
+    hx = h0
+    logps, ents, values = [], [], []
+    for t in range(obs.shape[0]):
+        logits, value, hx = policy(obs[t], mask[t], hx)
+        lp, ent = evaluate_actions(logits, actions[t])
+        logps.append(lp)
+        ents.append(ent)
+        values.append(value)
+        hx = hx * (1.0 - done[t].to(hx.dtype)).unsqueeze(-1)
+    return torch.stack(logps), torch.stack(ents), torch.stack(values)
 
 
 @dataclass
@@ -159,19 +181,9 @@ class PPOLearner:
             perm = torch.randperm(E, device=buf.obs.device)
             for i in range(cfg.minibatches):
                 ix = perm[i * mbe:(i + 1) * mbe]
-                hx = buf.h0[ix]
-                logps, ents, values = [], [], []
-                for t in range(T):
-                    logits, value, hx = self.policy(buf.obs[t, ix],
-                                                    buf.mask[t, ix], hx)
-                    lp, ent = evaluate_actions(logits, buf.actions[t, ix])
-                    logps.append(lp)
-                    ents.append(ent)
-                    values.append(value)
-                    hx = hx * (1.0 - buf.done[t, ix].to(hx.dtype)).unsqueeze(-1)
-                logp = torch.stack(logps)
-                entropy = torch.stack(ents)
-                value = torch.stack(values)
+                logp, entropy, value = replay_sequence(
+                    self.policy, buf.obs[:, ix], buf.mask[:, ix],
+                    buf.actions[:, ix], buf.h0[ix], buf.done[:, ix])
                 loss = self._loss(logp, entropy, value, buf.logp[:, ix],
                                   buf.value[:, ix], adv[:, ix], ret[:, ix],
                                   stats)
@@ -213,15 +225,8 @@ class A2CLearner:
         adv, ret = compute_gae(buf, cfg.gamma, cfg.lam)
         T, E = buf.reward.shape
         if self.policy.is_recurrent:
-            hx = buf.h0
-            logps, ents, values = [], [], []
-            for t in range(T):
-                logits, value, hx = self.policy(buf.obs[t], buf.mask[t], hx)
-                lp, ent = evaluate_actions(logits, buf.actions[t])
-                logps.append(lp); ents.append(ent); values.append(value)
-                hx = hx * (1.0 - buf.done[t].to(hx.dtype)).unsqueeze(-1)
-            logp, entropy, value = (torch.stack(logps), torch.stack(ents),
-                                    torch.stack(values))
+            logp, entropy, value = replay_sequence(
+                self.policy, buf.obs, buf.mask, buf.actions, buf.h0, buf.done)
         else:
             B = T * E
             logits, value, _ = self.policy(buf.obs.reshape(B, -1),

@@ -64,6 +64,9 @@ class Collector:
         self.obs = env.reset().to(torch.float32)
         self.mask = env.action_masks()
         self.hx = policy.initial_state(env.num_envs, self.device)
+        # policies with step() keep their state in place, and reset it
+        # themselves where the step before ended an episode
+        self.done_prev = None
         hidden = policy.hidden if policy.is_recurrent else 0
         self.buf = RolloutBuffer(T, env.num_envs, env.spec.obs_dim,
                                  env.spec.num_actions, self.device, hidden)
@@ -71,12 +74,21 @@ class Collector:
     @torch.no_grad()
     def collect(self) -> RolloutBuffer:
         buf = self.buf
+        in_place = hasattr(self.policy, "step")
         if buf.h0 is not None:
             buf.h0.copy_(self.hx)
+            if in_place and self.done_prev is not None:
+                buf.h0.masked_fill_(self.done_prev.bool().unsqueeze(-1), 0.0)
         for t in range(self.T):
             buf.obs[t].copy_(self.obs)
             buf.mask[t].copy_(self.mask)
-            logits, value, hx_next = self.policy(self.obs, self.mask, self.hx)
+            if in_place:
+                logits, value = self.policy.step(self.obs, self.mask, self.hx,
+                                                 self.done_prev)
+                hx_next = None
+            else:
+                logits, value, hx_next = self.policy(self.obs, self.mask,
+                                                     self.hx)
             u = torch.rand(self.env.num_envs, device=self.device,
                            generator=self.gen)
             a, lp, _ = sample_categorical(logits, u)
@@ -88,8 +100,14 @@ class Collector:
             buf.done[t].copy_(done)
             self.obs = obs.to(torch.float32)
             self.mask = info["action_mask"]
+            if in_place:
+                self.done_prev = done
             if hx_next is not None:
                 self.hx = hx_next * (1.0 - done.to(hx_next.dtype)).unsqueeze(-1)
-        _, last_v, _ = self.policy(self.obs, self.mask, self.hx)
+        if in_place:
+            _, last_v = self.policy.step(self.obs, self.mask, self.hx.clone(),
+                                         self.done_prev)
+        else:
+            _, last_v, _ = self.policy(self.obs, self.mask, self.hx)
         buf.last_value.copy_(last_v)
         return buf

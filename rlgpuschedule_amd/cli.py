@@ -16,6 +16,8 @@ def main(argv=None):
     sub = ap.add_subparsers(dest="cmd", required=True)
     tr = sub.add_parser("train", help="run a training config")
     tr.add_argument("--config", choices=sorted(CONFIGS), default="c2_ppo_mlp")
+    tr.add_argument("--policy", choices=["mlp", "gru", "linrec"],
+                    default=None, help="override the config's policy")
     tr.add_argument("--iterations", type=int, default=None)
     tr.add_argument("--envs", type=int, default=None)
     tr.add_argument("--rollout", type=int, default=None)
@@ -34,6 +36,9 @@ def main(argv=None):
                     help="2 = richer observations (docs/ENV_SPEC.md v4)")
     ev = sub.add_parser("eval", help="evaluate a checkpoint or baseline")
     ev.add_argument("--config", choices=sorted(CONFIGS), default="c2_ppo_mlp")
+    ev.add_argument("--policy", choices=["mlp", "gru", "linrec"],
+                    default=None, help="the checkpoint's policy, where it is "
+                    "not the config's")
     ev.add_argument("--ckpt", default=None, help="policy checkpoint (.pt/.safetensors)")
     ev.add_argument("--baseline", choices=["fifo", "sjf", "random"],
                     default=None)
@@ -74,6 +79,8 @@ def main(argv=None):
         import json
         from .agents.evaluate import evaluate_baseline, evaluate_policy
         cfg = CONFIGS[args.config]
+        if args.policy is not None:
+            cfg = dataclasses.replace(cfg, policy=args.policy)
         if args.trace_file:
             cfg = dataclasses.replace(
                 cfg, trace_kind="file",
@@ -121,6 +128,8 @@ def main(argv=None):
 
     cfg = CONFIGS[args.config]
     over = {}
+    if args.policy is not None:
+        over["policy"] = args.policy
     if args.envs is not None:
         over["num_envs"] = args.envs
     if args.rollout is not None:

@@ -12,7 +12,7 @@ from .agents.ppo import A2CConfig, A2CLearner, PPOConfig, PPOLearner
 from .agents.rollout import Collector, TorchEnvAdapter
 from .env.gym_api import CpuVectorEnv
 from .env.spec import EnvSpec, cluster16, cluster64, cluster256, cluster1024
-from .models.policy import GRUPolicy, MLPPolicy
+from .models.policy import GRUPolicy, LinearRecurrentPolicy, MLPPolicy
 from .parallel.dist import FlatGradAllreduce, broadcast_params, init_from_env
 
 
@@ -23,7 +23,7 @@ class TrainConfig:
     num_envs: int = 1024          # per GPU
     rollout_T: int = 64
     algo: str = "ppo"             # ppo | a2c | impala
-    policy: str = "mlp"           # mlp | gru
+    policy: str = "mlp"           # mlp | gru | linrec
     hidden: int = 256
     trace_kind: str = "philly"
     jobs_per_env: int = 256
@@ -90,7 +90,8 @@ def make_env(cfg: TrainConfig, device: torch.device, rank: int = 0):
 
 
 def make_policy(cfg: TrainConfig, device: torch.device):
-    cls = GRUPolicy if cfg.policy == "gru" else MLPPolicy
+    cls = {"gru": GRUPolicy, "linrec": LinearRecurrentPolicy}.get(
+        cfg.policy, MLPPolicy)
     pol = cls(cfg.spec.obs_dim, cfg.spec.num_actions, cfg.hidden)
     return pol.to(device)
 
@@ -122,6 +123,8 @@ def train(cfg: TrainConfig, iterations: int | None = None,
     if device.type == "cuda":
         device = torch.device(f"cuda:{local}")
     torch.manual_seed(cfg.seed * 31 + rank)
+    if cfg.policy == "linrec" and cfg.algo == "impala":
+        raise ValueError("policy='linrec' is trained by ppo and a2c")
     if cfg.algo == "impala":
         if callback is not None or solo:
             raise ValueError("algo='impala' does not support callback/solo "
@@ -149,7 +152,10 @@ def train(cfg: TrainConfig, iterations: int | None = None,
         if not solo:
             broadcast_params(policy)   # ranks cloned from different data
     grad_sync = FlatGradAllreduce(policy) if world > 1 else None
-    on_gpu_fast = device.type == "cuda" and cfg.use_hip_env
+    # the fused actors and learners know the MLP and the GRU; the linear
+    # recurrence acts and trains through its own kernels' autograd
+    on_gpu_fast = (device.type == "cuda" and cfg.use_hip_env
+                   and cfg.policy != "linrec")
     if on_gpu_fast:
         from .agents.rollout_gpu import GpuRolloutEngine
         collector = GpuRolloutEngine(env, policy, cfg.rollout_T,
