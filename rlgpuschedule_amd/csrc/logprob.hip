@@ -524,7 +524,7 @@ __global__ __launch_bounds__(kLanes) void logp_row_kernel(LogpFwd p,
 
 // The same for parts of up to kHeld vectors with alternatives, N of them in a
 // lane's registers: nothing is read twice.
-constexpr int kHeld = 4 * kLanes;
+constexpr int kHeld = 2 * kLanes;
 
 template <typename T, int N>
 __global__ __launch_bounds__(kLanes) void logp_part_kernel(LogpFwd p,
@@ -823,8 +823,6 @@ hipError_t fwd(const LogpFwd& p, void* scratch, int type, hipStream_t s) {
     e = launch(logp_row_kernel<T, false>, grid, lanes, 0, s, p, parts);
   } else if (n <= (int64_t)kLanes * P) {
     e = launch(logp_part_kernel<T, 1>, grid, lanes, 0, s, p, parts);
-  } else if (n <= 2 * (int64_t)kLanes * P) {
-    e = launch(logp_part_kernel<T, 2>, grid, lanes, 0, s, p, parts);
   } else if (n <= (int64_t)kHeld * P) {
     e = launch(logp_part_kernel<T, kHeld / kLanes>, grid, lanes, 0, s, p,
                parts);

@@ -6,6 +6,7 @@
 // few microseconds, and a backward pass written in Python spends more than
 // that on taking the interpreter's lock in autograd's thread.
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime_api.h>
 #include <pybind11/stl.h>
@@ -140,6 +141,7 @@ void refuse_foreign_leaves(const Tensor& t, const c10::hip::HIPStream& s,
       if (e.function) todo.push_back(e.function);
     if (node->num_outputs() != 0) continue;  // not a leaf's accumulation
     const auto at = node->stream();
+    if (at && at->device_type() == c10::kCPU) continue;
     if (at && (at->id() != s.id() || at->device_index() != s.device_index()))
       fail<std::runtime_error>(
           "an autograd graph of the same leaves, made on another stream, is "
@@ -468,7 +470,13 @@ Tensor scan_step(const Tensor& gate_, const Tensor& x_, Tensor h,
               "h is updated in place: it must be contiguous");
   VALUE_CHECK(!h.requires_grad() || !at::GradMode::is_enabled(),
               "h is updated in place and must not require a gradient");
+  for (const Tensor* t : {&gate_, &x_})
+    VALUE_CHECK(!h.is_alias_of(*t) || at::get_overlap_status(h, *t) ==
+                                          at::MemOverlapStatus::No,
+                "h is updated in place: it must not share memory with gate "
+                "or x");
   on_gpu(x_, "x");
+  h.unsafeGetTensorImpl()->bump_version();
   const int64_t E = x_.size(0), H = x_.size(1);
   Tensor hs = at::empty({E, H}, x_.options().requires_grad(false));
   const Tensor gate = reachable(gate_), x = reachable(x_);
@@ -479,7 +487,6 @@ Tensor scan_step(const Tensor& gate_, const Tensor& x_, Tensor h,
                               f32_ptr(h), out_ptr(hs), E, H, gate.stride(0),
                               x.stride(0), type),
             "rlsched_scan_step");
-  h.unsafeGetTensorImpl()->bump_version();
   return hs;
 }
 

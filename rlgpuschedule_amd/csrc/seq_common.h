@@ -6,6 +6,9 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <tuple>
+#include <type_traits>
+
 namespace seq {
 
 constexpr int kWave = 64;
@@ -152,7 +155,8 @@ template <typename... P, typename... A>
 inline hipError_t launch(void (*kernel)(P...), dim3 grid, dim3 block,
                          size_t lds, hipStream_t stream, A... args) {
   void* list[] = {(void*)&args...};
-  static_assert(sizeof...(P) == sizeof...(A), "one value for each parameter");
+  static_assert(std::is_same_v<std::tuple<P...>, std::tuple<A...>>,
+                "a value of its own type for each parameter");
   return hipLaunchKernel((const void*)kernel, grid, block, list, lds, stream);
 }
 

@@ -52,13 +52,16 @@ def gated_scan(gate: torch.Tensor, x: torch.Tensor,
 def gated_scan_step(gate: torch.Tensor, x: torch.Tensor, h: torch.Tensor,
                     done_prev: torch.Tensor | None = None) -> torch.Tensor:
     """One acting step: gate, x [E, H]; h [E, H] f32 contiguous, UPDATED IN
-    PLACE; done_prev [E] u8/bool marks environments whose state restarts from
-    zero before this step. Returns the output [E, H] in x's type. Not
+    PLACE and sharing no memory with the others; done_prev [E] u8/bool marks
+    environments whose state restarts from zero before this step. Returns the output [E, H] in x's type. Not
     differentiable."""
     if x.is_cuda:
         return ext().gated_scan_step(gate, x, h, done_prev)
     if not h.is_contiguous():
         raise ValueError("h is updated in place: it must be contiguous")
+    if h.requires_grad and torch.is_grad_enabled():
+        raise ValueError("h is updated in place and must not require a "
+                         "gradient")
     with torch.no_grad():
         c = h if done_prev is None else h.masked_fill(
             done_prev.unsqueeze(-1) != 0, 0.0)

@@ -432,6 +432,19 @@ def test_scan_step(device, dtype, E, H):
     close(h, *want["h_last"], "state")
 
 
+@pytest.mark.parametrize("device", DEVICES)
+def test_scan_step_in_inference_mode_and_version(device):
+    x = torch.randn(3, 8).to(device)
+    with torch.inference_mode():
+        h = torch.zeros(3, 8, device=device)
+        a = gated_scan_step(x.clone(), x.clone(), h)
+    g = torch.zeros(3, 8, device=device)
+    before = g._version
+    b = gated_scan_step(x, x, g)
+    assert torch.equal(a, b) and torch.equal(g, b)
+    assert g._version > before  # autograd sees the update
+
+
 def test_scan_refusals():
     x, h = torch.zeros(4, 2, 6), torch.zeros(2, 6)
     d = torch.zeros(4, 2, dtype=torch.uint8)
@@ -456,6 +469,9 @@ def test_scan_refusals():
         (ValueError, lambda: gated_scan_bwd(x, h, x, x, st)),
         (ValueError, lambda: ext().gated_scan_step(x[0], x[0], h.t(), None)),
         (ValueError, lambda: ext().gated_scan_step(x[0], x[0], h, None)),
+        (ValueError, lambda: ext().gated_scan_step(x[0], h, h, None)),
+        (ValueError, lambda: gated_scan_step(
+            x[0], x[0], h.clone().requires_grad_(True))),
         (ValueError, lambda: ext().gated_scan_step(
             x[0], x[0], h.clone().requires_grad_(True), None)),
         (ValueError, lambda: gated_scan_step(
