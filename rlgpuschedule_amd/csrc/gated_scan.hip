@@ -68,7 +68,8 @@ struct ScanFwd {
   void* hs;
   float* h_last;
   float* states;  // [ceil(T / kKeep), E, H]: c at t = 0, kKeep, ...; or null
-  float* carry;   // [chunks, E, H]: c at the chunks' starts; null: one chunk
+  const float* ways;  // [chunks, 2, E, H]: the chunks' effects, or null
+  float* carry;       // [chunks, E, H]: c at the chunks' starts, or null
   Cols c;
   int64_t T, chunk;
   int64_t gate_t, gate_e, x_t, x_e;  // strides of time and environment
@@ -84,7 +85,8 @@ struct ScanBwd {
   void* dgate;
   void* dx;
   float* dh0;    // null: not asked for
-  float* carry;  // [chunks, E, H]: a D of the step behind each chunk
+  const float* ways;  // [chunks, 2, E, H]: the chunks' effects, or null
+  float* carry;       // [chunks, E, H]: a D of the step behind each, or null
   Cols c;
   int64_t T, chunk;
   int64_t gate_t, gate_e, x_t, x_e, dhs_t, dhs_e;
@@ -117,6 +119,23 @@ struct Way {
     A = a < 0.f || A < 0.f ? -1.f : A * a;
   }
 };
+
+// A state's way through `count` chunks, from the `first` on or back.
+template <int V>
+__device__ __forceinline__ void follow(const float* ways, const Cols& cols,
+                                       const Lane& l, int64_t first, int count,
+                                       bool reverse, float (&c)[V]) {
+  const int64_t EH = cols.E * cols.H;
+#pragma unroll 4
+  for (int i = 0; i < count; ++i) {
+    const int64_t k = reverse ? first - i : first + i;
+    float A[V], B[V];
+    load<float, V>(here(ways + 2 * k * EH, l, cols.H), A);
+    load<float, V>(here(ways + (2 * k + 1) * EH, l, cols.H), B);
+#pragma unroll
+    for (int v = 0; v < V; ++v) c[v] = A[v] < 0.f ? B[v] : A[v] * c[v] + B[v];
+  }
+}
 
 // ---- forward
 // N steps of a lane's columns from t on. FULL: all of them are before `end`;
@@ -202,6 +221,7 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(ScanFwd p) {
   } else if (p.h0) {
     load<float, V>(here(p.h0, l, p.c.H), c);
   }
+  if (p.ways) follow<V>(p.ways, p.c, l, 0, blockIdx.y, false, c);
   if (t + L <= end) {
     // the next steps are read while these are walked
     Steps<T, V, L> s, n;
@@ -474,6 +494,9 @@ __global__ __launch_bounds__(256) void scan_bwd_kernel(ScanBwd p) {
   } else if (p.dh_last) {
     load<float, V>(here(p.dh_last, l, p.c.H), carry);
   }
+  if (p.ways)
+    follow<V>(p.ways, p.c, l, gridDim.y - 1, gridDim.y - 1 - blockIdx.y, true,
+              carry);
   int64_t t = t0 + (end - t0) / kKeep * kKeep;
   Sheet<T, V> now;
   if (t < end) {
@@ -554,20 +577,33 @@ struct Plan {
 constexpr int64_t kWaves = 4096;  // as many keep the memory busy
 constexpr int64_t kShort = 128;   // steps that one lane walks in any case
 
-// Lanes take 8 bytes of columns, or fewer where that leaves too few waves.
-Plan plan(int64_t T, int64_t E, int64_t H, int bytes) {
+// Lanes take 8 bytes of columns, as few load instructions as the memory's
+// rate allows, or fewer where that leaves too few waves: 64x256x256 bf16 runs
+// in 9.3 us forward and 18.8 us backward with 2 bytes, in 17.3 and 30.4 us
+// with 8; 64x1024x256 in 24 and 39 us with 8.
+//
+// Time is cut where a lane would walk more than kShort steps among few waves:
+// 512x32x256 bf16 runs in 17 and 24 us in chunks, in 47 and 106 us walked;
+// 129x32x256 fp32 in 11 and 14 us instead of 14 and 26. With 1024 waves it is
+// walked (256x1024x256 bf16: 92 and 164 us, in chunks 162 and 241, which read
+// more), but backward not by lanes of 2 bytes (512x256x256 bf16: 64 us walked
+// forward, 75 in chunks; 134 us walked backward, 109 in chunks).
+Plan plan(int64_t T, int64_t E, int64_t H, int bytes, bool back) {
   Plan p;
   int64_t waves = 0;
-  for (p.V = 8 / bytes; p.V >= 1; p.V /= 2) {
-    if (p.V > H) continue;
-    p.n = (H + p.V - 1) / p.V;
-    waves = (E * p.n + kWave - 1) / kWave;
-    const int64_t cuts = T > kShort ? T / 64 : 1;
-    if (p.V == 1 || waves * cuts >= kWaves / 4) break;
-  }
+  auto lay = [&](int64_t cuts) {
+    for (p.V = 8 / bytes; p.V >= 1; p.V /= 2) {
+      if (p.V > H) continue;
+      p.n = (H + p.V - 1) / p.V;
+      waves = (E * p.n + kWave - 1) / kWave;
+      if (p.V == 1 || waves * cuts >= kWaves / 4) break;
+    }
+  };
+  lay(1);
   p.chunk = T;
   p.chunks = 1;
-  if (T > kShort && waves < kWaves / 2) {
+  if (T > kShort && (waves < kWaves / 4 || (back && p.V * bytes < 4))) {
+    lay(T / 64);
     int64_t want = kWaves / waves;  // chunks
     const int64_t most = (T + 15) / 16;
     want = want < most ? want : most;
@@ -581,9 +617,18 @@ Plan plan(int64_t T, int64_t E, int64_t H, int bytes) {
   return p;
 }
 
-// scratch: the chunks' ways and their carries
-float* carry_of(const Plan& q, float* scratch, int64_t EH) {
-  return q.chunks > 1 ? scratch + 2 * q.chunks * EH : nullptr;
+// A chunk follows the ways of up to kFollow others itself, without a kernel
+// between: 509x37x263 fp16's 22 chunks are walked 4 us sooner each way. More
+// would read too much: scratch then holds the chunks' starts as well.
+constexpr int64_t kFollow = 32;
+
+template <typename P>
+void give_ways(P& p, const Plan& q, float* scratch) {
+  const int64_t EH = p.c.E * p.c.H;
+  p.c.n = q.n;
+  p.chunk = q.chunk;
+  p.ways = q.chunks > 1 && q.chunks <= kFollow ? scratch : nullptr;
+  p.carry = q.chunks > kFollow ? scratch + 2 * q.chunks * EH : nullptr;
 }
 
 hipError_t join(const float* ways, const float* first, float* carry,
@@ -601,7 +646,8 @@ hipError_t fwd_with(const ScanFwd& p, const Plan& q, float* ways,
   if (q.chunks > 1) {
     hipError_t e = launch(scan_fwd_way_kernel<T, V, DONE>, grid, dim3(256), 0, s,
                           p, ways);
-    if (e == hipSuccess) e = join(ways, p.h0, p.carry, q, EH, false, s);
+    if (e == hipSuccess && p.carry)
+      e = join(ways, p.h0, p.carry, q, EH, false, s);
     if (e != hipSuccess) return e;
   }
   return launch(scan_fwd_kernel<T, V, kKeep, DONE>, grid, dim3(256), 0, s, p);
@@ -610,10 +656,8 @@ hipError_t fwd_with(const ScanFwd& p, const Plan& q, float* ways,
 template <typename T>
 hipError_t fwd(ScanFwd p, float* scratch, hipStream_t s) {
   if (p.c.E * p.c.H == 0) return hipSuccess;
-  const Plan q = plan(p.T, p.c.E, p.c.H, sizeof(T));
-  p.c.n = q.n;
-  p.chunk = q.chunk;
-  p.carry = carry_of(q, scratch, p.c.E * p.c.H);
+  const Plan q = plan(p.T, p.c.E, p.c.H, sizeof(T), false);
+  give_ways(p, q, scratch);
   switch (q.V * 2 + (p.done != nullptr)) {
     case 2: return fwd_with<T, 1, false>(p, q, scratch, s);
     case 3: return fwd_with<T, 1, true>(p, q, scratch, s);
@@ -635,7 +679,8 @@ hipError_t bwd_with(const ScanBwd& p, const Plan& q, float* ways,
   if (q.chunks > 1) {
     hipError_t e =
         launch(scan_bwd_way_kernel<T, V, DONE>, grid, dim3(256), 0, s, p, ways);
-    if (e == hipSuccess) e = join(ways, p.dh_last, p.carry, q, EH, true, s);
+    if (e == hipSuccess && p.carry)
+      e = join(ways, p.dh_last, p.carry, q, EH, true, s);
     if (e != hipSuccess) return e;
   }
   return launch(scan_bwd_kernel<T, V, DONE>, grid, dim3(256), 0, s, p);
@@ -644,10 +689,8 @@ hipError_t bwd_with(const ScanBwd& p, const Plan& q, float* ways,
 template <typename T>
 hipError_t bwd(ScanBwd p, float* scratch, hipStream_t s) {
   if (p.c.E * p.c.H == 0) return hipSuccess;
-  const Plan q = plan(p.T, p.c.E, p.c.H, sizeof(T));
-  p.c.n = q.n;
-  p.chunk = q.chunk;
-  p.carry = carry_of(q, scratch, p.c.E * p.c.H);
+  const Plan q = plan(p.T, p.c.E, p.c.H, sizeof(T), true);
+  give_ways(p, q, scratch);
   switch (q.V * 2 + (p.done != nullptr)) {
     case 2: return bwd_with<T, 1, false>(p, q, scratch, s);
     case 3: return bwd_with<T, 1, true>(p, q, scratch, s);
@@ -663,12 +706,13 @@ hipError_t bwd(ScanBwd p, float* scratch, hipStream_t s) {
 
 }  // namespace
 
-// Floats of scratch that the forward and the backward call each need.
+// Floats of scratch that the forward or the backward call needs.
 extern "C" int64_t rlsched_scan_scratch(int64_t T, int64_t E, int64_t H,
-                                        int type) {
+                                        int type, int back) {
   if (E * H == 0) return 0;
-  const Plan q = plan(T, E, H, type == F32 ? 4 : 2);
-  return q.chunks > 1 ? 3 * q.chunks * E * H : 0;
+  const Plan q = plan(T, E, H, type == F32 ? 4 : 2, back);
+  if (q.chunks == 1) return 0;
+  return (q.chunks > kFollow ? 3 : 2) * q.chunks * E * H;
 }
 
 // Elements from one environment to the next that a lane's 32-bit distance
@@ -691,8 +735,9 @@ extern "C" int rlsched_scan_fwd(int device, void* stream, const void* gate,
                                 int type) {
   OnDevice on(device);
   if (on.err != hipSuccess) return on.err;
-  const ScanFwd p = {gate,   x, h0, done, hs, h_last, states, nullptr,
-                     {E, H}, T, 0,  gate_t, gate_e, x_t, x_e};
+  const ScanFwd p = {gate,    x,       h0,     done, hs, h_last, states,
+                     nullptr, nullptr, {E, H}, T,    0,  gate_t, gate_e,
+                     x_t,     x_e};
   const hipStream_t s = (hipStream_t)stream;
   if (type == F32) return fwd<float>(p, scratch, s);
   if (type == BF16) return fwd<bf16>(p, scratch, s);
@@ -710,9 +755,9 @@ extern "C" int rlsched_scan_bwd(int device, void* stream, const void* dhs,
                                 int64_t dhs_t, int64_t dhs_e, int type) {
   OnDevice on(device);
   if (on.err != hipSuccess) return on.err;
-  const ScanBwd p = {dhs, dh_last, gate,    x,      states, done, dgate,
-                     dx,  dh0,     nullptr, {E, H}, T,      0,    gate_t,
-                     gate_e, x_t,  x_e,     dhs_t,  dhs_e};
+  const ScanBwd p = {dhs, dh_last, gate,    x,       states, done,  dgate,
+                     dx,  dh0,     nullptr, nullptr, {E, H}, T,     0,
+                     gate_t, gate_e, x_t,   x_e,     dhs_t,  dhs_e};
   const hipStream_t s = (hipStream_t)stream;
   if (type == F32) return bwd<float>(p, scratch, s);
   if (type == BF16) return bwd<bf16>(p, scratch, s);

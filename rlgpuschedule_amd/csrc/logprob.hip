@@ -797,10 +797,12 @@ hipError_t group(const P& p, hipStream_t s) {
 
 // Parts of a row: of 512 vectors at least, while there are fewer blocks than
 // keep the chip busy; with alternatives of as many as registers hold at most.
+constexpr int64_t kBlocks = 512;
+
 int parts_of(int64_t rows, int64_t A, int k, int V) {
   const int64_t n = (A + V - 1) / V;
   if (n <= group_vecs(k) || rows <= 0) return 1;
-  int64_t p = (1024 + rows - 1) / rows;
+  int64_t p = (kBlocks + rows - 1) / rows;
   p = p < n / 512 ? p : n / 512;
   if (k && p < (n + kHeld - 1) / kHeld) p = (n + kHeld - 1) / kHeld;
   p = p < kMostParts ? p : kMostParts;

@@ -17,7 +17,8 @@ int rlsched_norm_bwd(int device, void* stream, const void* dy, const void* x,
                      int64_t rows, int64_t dim, int64_t x_stride,
                      int64_t dy_stride, int type, int wtype);
 
-int64_t rlsched_scan_scratch(int64_t T, int64_t E, int64_t H, int type);
+int64_t rlsched_scan_scratch(int64_t T, int64_t E, int64_t H, int type,
+                             int back);
 int64_t rlsched_scan_states(int64_t T);
 int64_t rlsched_scan_reach(int64_t H);
 int rlsched_scan_fwd(int device, void* stream, const void* gate, const void* x,

@@ -362,7 +362,7 @@ std::tuple<Tensor, Tensor, Tensor> scan_fwd(const Tensor& gate_,
   Tensor h_last = f32(x_, {E, H}), states;
   if (keep) states = f32(x_, {rlsched_scan_states(T), E, H});
   Tensor scratch;
-  if (const int64_t n = rlsched_scan_scratch(T, E, H, type))
+  if (const int64_t n = rlsched_scan_scratch(T, E, H, type, 0))
     scratch = f32(x_, {n});
   const Tensor gate = reachable(gate_), x = reachable(x_);
   const MaybeTensor h0 = packed(h0_), done = packed(done_);
@@ -402,7 +402,7 @@ std::tuple<Tensor, Tensor, Tensor> scan_bwd(
   Tensor dx = at::empty({T, E, H}, like_x), dh0;
   if (need_dh0) dh0 = f32(x_, {E, H});
   Tensor scratch;
-  if (const int64_t n = rlsched_scan_scratch(T, E, H, type))
+  if (const int64_t n = rlsched_scan_scratch(T, E, H, type, 1))
     scratch = f32(x_, {n});
   const Tensor gate = reachable(gate_), x = reachable(x_);
   MaybeTensor dhs;
