@@ -14,15 +14,25 @@
 // A lane owns V neighbouring columns of one environment and walks time. With
 // columns enough for the chip it walks all of it, in one pass. With fewer,
 // time is cut into chunks: a first kernel finds each chunk's effect on the
-// state, c_end = A c_start + B, a second joins those from chunk to chunk,
-// and a third walks every chunk from its own start.
+// state, c_end = A c_start + B, those are joined from chunk to chunk, and a
+// last kernel walks every chunk from its own start.
+//
+// Bound by memory where it is walked: 64 x 2048 x 256 bf16 takes 46 us forward
+// (217 MB with the kept states, 4.7 TB/s) and 70 us backward (352 MB, 5.0), a
+// large copy's rate being 4.9. In chunks gate and x are read twice: 32768 x 2
+// x 1000 takes 70 us for the effects (262 MB; reading alone runs at 4.0 TB/s),
+// 12 to join 512 chunks and 64 to walk. Small calls are bound by the latency
+// of kKeep steps after another: 65 x 64 x 256 bf16 takes 7.5 and 11 us.
 #include "seq_api.h"
 #include "seq_common.h"
 
 namespace {
 using namespace seq;
 
-constexpr int kKeep = 8;  // steps from one kept state to the next
+// Steps from one kept state to the next: what the backward pass holds at once.
+// 16 of them took twice the registers for half as wide loads: 128 us instead
+// of 112 for a training pass of 64 x 2048 x 256 bf16.
+constexpr int kKeep = 8;
 
 // A sequence's columns as lanes: n lanes an environment, the last of which
 // begins early enough to end with it and computes shared columns twice, to
@@ -575,7 +585,7 @@ struct Plan {
 };
 
 constexpr int64_t kWaves = 4096;  // as many keep the memory busy
-constexpr int64_t kShort = 128;   // steps that one lane walks in any case
+constexpr int64_t kShort = 64;    // steps that one lane walks in any case
 
 // Lanes take 8 bytes of columns, as few load instructions as the memory's
 // rate allows, or fewer where that leaves too few waves: 64x256x256 bf16 runs
@@ -583,8 +593,9 @@ constexpr int64_t kShort = 128;   // steps that one lane walks in any case
 // with 8; 64x1024x256 in 24 and 39 us with 8.
 //
 // Time is cut where a lane would walk more than kShort steps among few waves:
-// 512x32x256 bf16 runs in 17 and 24 us in chunks, in 47 and 106 us walked;
-// 129x32x256 fp32 in 11 and 14 us instead of 14 and 26. With 1024 waves it is
+// 512x32x256 bf16 runs in 14 and 22 us in chunks, in 47 and 106 us walked;
+// 65x64x256 in 7.5 and 11 us instead of 9 and 16; 32x64x64 fp32 would take 6.6
+// and 9.4 instead of 5.0 and 8.6. With 1024 waves it is
 // walked (256x1024x256 bf16: 92 and 164 us, in chunks 162 and 241, which read
 // more), but backward not by lanes of 2 bytes (512x256x256 bf16: 64 us walked
 // forward, 75 in chunks; 134 us walked backward, 109 in chunks).

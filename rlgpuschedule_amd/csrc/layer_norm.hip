@@ -7,6 +7,12 @@
 //
 // Statistics and sums are held in 32 bits; y, dx, dw and db are rounded to
 // their types once.
+//
+// Bound by memory: x is read once by each pass and held in registers between
+// the sums and what needs them, dy likewise. On an MI355X, whose large copy
+// runs at 4.9 TB/s, 131072 x 256 bf16 takes 27 us forward (5.0 TB/s) and 37
+// us backward (5.5 TB/s, the last sum among it), 8192 x 4096 fp16 26 and 44
+// us; 256 x 256 fp32 takes 2.7 us, a launch's time.
 #include "seq_api.h"
 #include "seq_common.h"
 
@@ -203,6 +209,8 @@ __global__ __launch_bounds__(kBlock<G>) void norm_fwd_kernel(NormFwd p) {
 
 // dx of a block's rows, and the rows' share of dw and db: the lanes keep
 // theirs in registers over all rows, then the block's row groups are added.
+// No atomics: the order of the sums is the same each time. A share is written
+// and read once more, 4 us of 131072 x 256's 37.
 template <typename T, int G, int N>
 __global__ __launch_bounds__(kBlock<G>) void norm_bwd_kernel(NormBwd p) {
   constexpr int V = kVec<T>, R = kBlock<G> / G;
@@ -419,6 +427,10 @@ __global__ __launch_bounds__(32 * kSumLanes) void norm_sum_kernel(NormSum a) {
 constexpr int64_t kGrid = 1 << 22;  // blocks at most; more rows are looped over
 
 // How a row lies on lanes: G of them with N vectors each; G = 0: too long.
+// Two vectors a lane, for twice the bytes in flight: with one, 131072 x 256
+// bf16 took 29 us forward and 47 backward, 32768 x 1024 28 and 72. A row of
+// more than 2048 vectors would not leave registers for its share of dw and db:
+// it is walked and read again.
 struct Shape {
   int G, N;
 };
@@ -431,6 +443,9 @@ Shape shape_of(int64_t dim, int bytes) {
   return {0, 0};
 }
 
+// Blocks of the backward pass, each with a share: 2048 to 4096 waves, which is
+// what 128 registers a lane leave room for. Fewer wide ones for fewer shares
+// gain nothing: 5003 x 1021 fp32 takes 22 us with 625 as with 1024 of them.
 int parts_of(int64_t rows, int64_t dim, int bytes) {
   const Shape s = shape_of(dim, bytes);
   const int64_t at_once = s.G == 0 ? 32 : s.G <= kWave ? 512 / s.G : 1;
