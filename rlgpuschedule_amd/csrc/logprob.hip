@@ -64,6 +64,11 @@ __device__ __forceinline__ float value_of(uint64_t key) {
 __device__ __forceinline__ int64_t index_of(uint64_t key) {
   return (int64_t)(0xffffffffu - (uint32_t)key);
 }
+
+__device__ __forceinline__ uint64_t larger(uint64_t a, uint64_t b) {
+  return a > b ? a : b;
+}
+
 // Vector j of a row. The last vector of a row of no whole number of them
 // begins early enough to end with the row; what it shares with the one
 // before is left out unless SHARED, so no element is counted twice.
@@ -205,13 +210,6 @@ __device__ __forceinline__ int rank_of(uint64_t mine, const uint64_t* keys,
   return rank;
 }
 
-// ---- rows of up to G * N vectors: G lanes a row, all of it in registers
-// Few lanes with up to four vectors each share a row's bookkeeping among few:
-// 524288 x 17 fp32 takes 17 us with 2 lanes of 3 vectors, 25 with 8 of one.
-__device__ __forceinline__ uint64_t larger(uint64_t a, uint64_t b) {
-  return a > b ? a : b;
-}
-
 // A lower bound of the k-th largest element, from 64 lanes' or groups' bests,
 // no element the best of two: the least that fewer than k are above. At least
 // the lowest finite value. For one wave; the result is in all its lanes.
@@ -252,6 +250,9 @@ __device__ __forceinline__ uint64_t key_at(float v, int l, int at, int A) {
   return v > -INFINITY ? key_of(v, from + at % V) : 0;
 }
 
+// ---- rows of up to G * N vectors: G lanes a row, all of it in registers
+// Few lanes with up to four vectors each share a row's bookkeeping among few:
+// 524288 x 17 fp32 takes 17 us with 2 lanes of 3 vectors, 25 with 8 of one.
 template <typename T, int G, int N, bool TOP>
 __global__ __launch_bounds__(256) void logp_group_kernel(LogpFwd p) {
   constexpr int V = kVec<T>, R = 256 / G;
@@ -359,7 +360,8 @@ struct Running {
 };
 
 constexpr int kLanes = 256;
-constexpr int kFound = 256;  // alternatives that are sorted out at once
+// Elements that are ranked at once: of 64 bests' least about 300 are above.
+constexpr int kFound = 512;
 
 // least_of a block's lanes, four of which have a head. `count` is cleared.
 __device__ __forceinline__ float block_least(float own, int k, float* heads,

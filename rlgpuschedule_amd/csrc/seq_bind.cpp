@@ -494,8 +494,8 @@ Tensor scan_step(const Tensor& gate_, const Tensor& x_, Tensor h,
 int check_logp(const Tensor& logits, const Tensor& actions,
                const MaybeTensor& mask, int64_t top_k) {
   VALUE_CHECK(logits.dim() >= 1 && logits.size(-1) > 0 &&
-                  logits.size(-1) < (1ll << 31),
-              "logits must have 1 to 2**31 - 1 actions, got shape ",
+                  logits.size(-1) <= (1ll << 30),
+              "logits must have 1 to 2**30 actions, got shape ",
               logits.sizes());
   const int code = type_code(logits, "logits");
   const auto lead = logits.sizes().slice(0, logits.dim() - 1);

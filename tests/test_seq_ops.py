@@ -586,7 +586,7 @@ def check_logp(logits, actions, mask, top_k, dlogp, dent, what=""):
 LOGP_SIZES = [(1, 1), (3, 2), (50, 5), (300, 17), (5, 21), (70, 64), (33, 65),
               (9, 100), (4, 256), (7, 1000), (3, 1024), (5, 4097), (2, 8192),
               (2, 10007), (1, 20000), (1, 70000), (3, 32768),
-              (2, 600007)]
+              (2, 600007), (3, 3000), (40, 1030)]
 
 
 @pytest.mark.parametrize("device", DEVICES)
@@ -707,6 +707,8 @@ def test_logp_refusals():
     cases = [
         (ValueError, lambda: action_logprobs_fwd(torch.zeros(()), a)),
         (ValueError, lambda: action_logprobs_fwd(torch.zeros(4, 0), a)),
+        (ValueError, lambda: action_logprobs_fwd(
+            torch.zeros(1).expand(4, (1 << 30) + 1), a)),
         (TypeError, lambda: action_logprobs_fwd(x.double(), a)),
         (ValueError, lambda: action_logprobs_fwd(x, a[:3])),
         (ValueError, lambda: action_logprobs_fwd(x, a.int())),
