@@ -90,8 +90,14 @@ void* out_ptr(const Tensor& t) {
   return t.defined() ? t.mutable_data_ptr() : nullptr;
 }
 float* f32_ptr(const Tensor& t) { return (float*)out_ptr(t); }
+MaybeTensor maybe(const Tensor& t) {
+  return t.defined() ? MaybeTensor(t) : std::nullopt;
+}
+// Values as memory holds them: torch notes a conjugate's imaginary part as to
+// be negated.
 MaybeTensor packed(const MaybeTensor& t) {
-  return t && t->defined() ? MaybeTensor(t->contiguous()) : std::nullopt;
+  return t && t->defined() ? MaybeTensor(t->resolve_neg().contiguous())
+                           : std::nullopt;
 }
 
 Tensor f32(const Tensor& x, at::IntArrayRef size) {
@@ -101,7 +107,8 @@ Tensor f32(const Tensor& x, at::IntArrayRef size) {
 // t [..., D] as rows of unit stride and the elements from one row to the
 // next. Leading dims that no single stride walks, and last dims of another
 // stride, are copied.
-std::pair<Tensor, int64_t> rows_of(const Tensor& t) {
+std::pair<Tensor, int64_t> rows_of(const Tensor& t_) {
+  const Tensor t = t_.resolve_neg();
   const int64_t d = t.size(-1);
   if (t.is_contiguous()) return {t, d};
   Tensor r = t.reshape({-1, d});
@@ -110,7 +117,8 @@ std::pair<Tensor, int64_t> rows_of(const Tensor& t) {
 }
 
 // t [..., E, H] with neighbouring columns and environments within reach.
-Tensor reachable(const Tensor& t) {
+Tensor reachable(const Tensor& t_) {
+  const Tensor t = t_.resolve_neg();
   const bool near = t.stride(-2) <= rlsched_scan_reach(t.size(-1));
   const bool unit = t.size(-1) == 1 || t.stride(-1) == 1;
   return near && unit ? t : t.contiguous();
@@ -165,6 +173,14 @@ void check_capture(const Tensor& x, const T&... rest) {
   visit(x);
   (visit(MaybeTensor(rest)), ...);
 }
+
+// Forward-mode derivatives would be dropped where nothing requires a gradient.
+void no_tangent(const char* name, std::initializer_list<const Tensor*> all) {
+  for (const Tensor* t : all)
+    if (t && t->_fw_grad(0).defined())
+      fail<std::runtime_error>(name, " has no forward-mode derivative");
+}
+const Tensor* given(const MaybeTensor& t) { return t ? &*t : nullptr; }
 
 void once(const char* name) {
   if (at::GradMode::is_enabled())
@@ -309,6 +325,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
 
 Tensor layer_norm(const Tensor& x, const MaybeTensor& weight,
                   const MaybeTensor& bias, double eps) {
+  no_tangent("layer_norm", {&x, given(weight), given(bias)});
   if (at::GradMode::is_enabled() &&
       (wants_grad(x) || wants_grad(weight) || wants_grad(bias))) {
     check_norm(x, weight, bias);
@@ -437,13 +454,10 @@ struct GatedScan : torch::autograd::Function<GatedScan> {
     if (!grads[0].defined() && !grads[1].defined())
       return {Tensor(), Tensor(), Tensor(), Tensor()};
     const auto s = ctx->get_saved_variables();
-    auto given = [](const Tensor& t) {
-      return t.defined() ? MaybeTensor(t) : std::nullopt;
-    };
     const bool need_dh0 =
         ctx->saved_data["h0"].toBool() && ctx->needs_input_grad(2);
-    auto [dgate, dx, dh0] = scan_bwd(given(grads[0]), given(grads[1]), s[0],
-                                     s[1], s[2], given(s[3]), need_dh0);
+    auto [dgate, dx, dh0] = scan_bwd(maybe(grads[0]), maybe(grads[1]), s[0],
+                                     s[1], s[2], maybe(s[3]), need_dh0);
     return {dgate, dx, dh0, Tensor()};
   }
 };
@@ -451,6 +465,7 @@ struct GatedScan : torch::autograd::Function<GatedScan> {
 std::tuple<Tensor, Tensor> gated_scan(const Tensor& gate, const Tensor& x,
                                       const MaybeTensor& h0,
                                       const MaybeTensor& done) {
+  no_tangent("gated_scan", {&gate, &x, given(h0)});
   if (at::GradMode::is_enabled() &&
       (wants_grad(gate) || wants_grad(x) || wants_grad(h0))) {
     check_scan(gate, x, h0, done, 3, "h0");
@@ -466,15 +481,15 @@ std::tuple<Tensor, Tensor> gated_scan(const Tensor& gate, const Tensor& x,
 Tensor scan_step(const Tensor& gate_, const Tensor& x_, Tensor h,
                  const MaybeTensor& done_) {
   const int type = check_scan(gate_, x_, h, done_, 2, "h");
-  VALUE_CHECK(h.is_contiguous(),
+  VALUE_CHECK(h.is_contiguous() && !h.is_neg(),
               "h is updated in place: it must be contiguous");
   VALUE_CHECK(!h.requires_grad() || !at::GradMode::is_enabled(),
               "h is updated in place and must not require a gradient");
-  for (const Tensor* t : {&gate_, &x_})
-    VALUE_CHECK(!h.is_alias_of(*t) || at::get_overlap_status(h, *t) ==
-                                          at::MemOverlapStatus::No,
-                "h is updated in place: it must not share memory with gate "
-                "or x");
+  for (const Tensor* t : {&gate_, &x_, given(done_)})
+    VALUE_CHECK(!t || !h.is_alias_of(*t) ||
+                    at::get_overlap_status(h, *t) == at::MemOverlapStatus::No,
+                "h is updated in place: it must not share memory with gate, "
+                "x or done");
   on_gpu(x_, "x");
   h.unsafeGetTensorImpl()->bump_version();
   const int64_t E = x_.size(0), H = x_.size(1);
@@ -612,10 +627,7 @@ struct ActionLogProbs : torch::autograd::Function<ActionLogProbs> {
     if (!grads[0].defined() && !grads[1].defined())
       return {Tensor(), Tensor(), Tensor(), Tensor()};
     const auto s = ctx->get_saved_variables();
-    auto given = [](const Tensor& t) {
-      return t.defined() ? MaybeTensor(t) : std::nullopt;
-    };
-    return {logp_bwd(given(grads[0]), given(grads[1]), s[0], s[1], given(s[2]),
+    return {logp_bwd(maybe(grads[0]), maybe(grads[1]), s[0], s[1], maybe(s[2]),
                      s[3]),
             Tensor(), Tensor(), Tensor()};
   }
@@ -624,6 +636,7 @@ struct ActionLogProbs : torch::autograd::Function<ActionLogProbs> {
 std::tuple<Tensor, Tensor, MaybeTensor, MaybeTensor> action_logprobs(
     const Tensor& logits, const Tensor& actions, const MaybeTensor& mask,
     int64_t top_k) {
+  no_tangent("action_logprobs", {&logits});
   if (at::GradMode::is_enabled() && logits.requires_grad()) {
     check_logp(logits, actions, mask, top_k);
     on_gpu(logits, "logits");
@@ -636,10 +649,6 @@ std::tuple<Tensor, Tensor, MaybeTensor, MaybeTensor> action_logprobs(
       logp_fwd(logits, actions, mask, top_k, false);
   if (!top_k) return {logp, entropy, std::nullopt, std::nullopt};
   return {logp, entropy, tl, ti};
-}
-
-MaybeTensor maybe(const Tensor& t) {
-  return t.defined() ? MaybeTensor(t) : std::nullopt;
 }
 
 }  // namespace

@@ -31,8 +31,8 @@ class LogProbs(NamedTuple):
 def action_logprobs_fwd(logits: torch.Tensor, actions: torch.Tensor,
                         mask: torch.Tensor | None = None, top_k: int = 0):
     """logits [..., A] on a GPU (float32, bfloat16 or float16, any row
-    stride, at most 2**30 actions), actions [...] i64, mask [..., A] u8/bool (nonzero: allowed) or
-    None. Returns (logp, entropy [...] f32, stats [rows, 3] f32, top_logp,
+    stride, at most 2**30 actions), actions [...] i64, mask [..., A] u8/bool
+    (nonzero: allowed) or None. Returns (logp, entropy [...] f32, stats [rows, 3] f32, top_logp,
     top_index): see action_logprobs; stats is what action_logprobs_bwd needs."""
     return ext().action_logprobs_fwd(logits, actions, mask, top_k)
 

@@ -53,8 +53,8 @@ def gated_scan_step(gate: torch.Tensor, x: torch.Tensor, h: torch.Tensor,
                     done_prev: torch.Tensor | None = None) -> torch.Tensor:
     """One acting step: gate, x [E, H]; h [E, H] f32 contiguous, UPDATED IN
     PLACE and sharing no memory with the others; done_prev [E] u8/bool marks
-    environments whose state restarts from zero before this step. Returns the output [E, H] in x's type. Not
-    differentiable."""
+    environments whose state restarts from zero before this step. Returns the
+    output [E, H] in x's type. Not differentiable."""
     if x.is_cuda:
         return ext().gated_scan_step(gate, x, h, done_prev)
     if not h.is_contiguous():

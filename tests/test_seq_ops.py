@@ -470,6 +470,8 @@ def test_scan_refusals():
         (ValueError, lambda: ext().gated_scan_step(x[0], x[0], h.t(), None)),
         (ValueError, lambda: ext().gated_scan_step(x[0], x[0], h, None)),
         (ValueError, lambda: ext().gated_scan_step(x[0], h, h, None)),
+        (ValueError, lambda: ext().gated_scan_step(
+            x[0], x[0], h, h.view(torch.uint8).view(-1)[:2])),
         (ValueError, lambda: gated_scan_step(
             x[0], x[0], h.clone().requires_grad_(True))),
         (ValueError, lambda: ext().gated_scan_step(
@@ -943,6 +945,72 @@ def test_second_derivatives_are_refused():
               action_logprobs(x, act).logp):
         with pytest.raises(RuntimeError, match="create_graph"):
             torch.autograd.grad(y.sum(), x, create_graph=True)
+
+
+def test_forward_mode_is_refused():
+    x = torch.randn(4, 3, 8)
+    act = torch.zeros(4, 3, dtype=torch.int64)
+    with torch.autograd.forward_ad.dual_level():
+        d = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        for call in (lambda: ext().layer_norm(d, None, None, 1e-5),
+                     lambda: ext().layer_norm(x, d[0, 0], None, 1e-5),
+                     lambda: ext().gated_scan(d, x, None, None),
+                     lambda: ext().gated_scan(x, x, d[0], None),
+                     lambda: ext().action_logprobs(d, act, None, 0)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+
+
+@pytest.mark.gpu
+def test_backward_twice_and_from_threads():
+    """A kept graph gives the same gradients again, and graphs of the same
+    leaves that threads make and walk at once give each what it would get
+    alone."""
+    import threading
+    x = torch.randn(37, 5, 24, device="cuda", requires_grad=True)
+    w = torch.randn(24, device="cuda", requires_grad=True)
+    act = torch.randint(0, 24, (37, 5), device="cuda")
+
+    def loss():
+        n = layer_norm(x, w)
+        hs, last = gated_scan(n, x)
+        r = action_logprobs(hs, act)
+        return r.logp.sum() + r.entropy.square().sum() + last.sum()
+
+    y = loss()
+    want = torch.autograd.grad(y, (x, w), retain_graph=True)
+    assert same(torch.autograd.grad(y, (x, w)), want)
+    torch.cuda.synchronize()
+    got = [None] * 4
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(5):
+                got[i] = torch.autograd.grad(loss(), (x, w))
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for i in range(4):
+        assert same(got[i], want), i
+
+
+@pytest.mark.gpu
+def test_negated_views():
+    """An imaginary part of a conjugate holds its values negated."""
+    c = torch.randn(6, 5, 8, dtype=torch.complex64, device="cuda")
+    v, h = c.conj().imag, c[0].conj().imag
+    p = v.resolve_neg().contiguous()
+    act = torch.zeros(6, 5, dtype=torch.int64, device="cuda")
+    assert v.is_neg()
+    assert torch.equal(layer_norm(v, v[0, 0], v[0, 1]),
+                       layer_norm(p, p[0, 0], p[0, 1]))
+    assert same(gated_scan(v, v, h), gated_scan(p, p, p[0]))
+    assert same(action_logprobs(v, act)[:2], action_logprobs(p, act)[:2])
 
 
 @pytest.mark.gpu
