@@ -145,19 +145,26 @@ __device__ __forceinline__ void finish_row(const LogpFwd& p, int64_t row,
   }
 }
 
-__device__ __forceinline__ void finish_top(const LogpFwd& p, int64_t row,
-                                           int j, uint64_t key, float m,
-                                           float s) {
-  const bool broken = s != s;
-  float lp = -INFINITY;
-  int64_t ix = -1;
-  if (key && !broken) {
-    lp = value_of(key) - m - logf(s);
-    ix = index_of(key);
+// Where a row's alternatives go.
+struct Top {
+  float* logp;
+  int64_t* index;
+  float m, ls;
+  bool broken;
+
+  __device__ __forceinline__ Top(const LogpFwd& p, int64_t row, float m_,
+                                 float s)
+      : logp(p.top_logp + row * p.k),
+        index(p.top_index + row * p.k),
+        m(m_),
+        ls(logf(s)),
+        broken(s != s) {}
+  __device__ __forceinline__ void put(int rank, uint64_t key) const {
+    const bool some = key && !broken;
+    logp[rank] = broken ? NAN : some ? value_of(key) - m - ls : -INFINITY;
+    index[rank] = some ? index_of(key) : -1;
   }
-  p.top_logp[row * p.k + j] = broken ? NAN : lp;
-  p.top_index[row * p.k + j] = ix;
-}
+};
 
 template <typename T>
 __device__ __forceinline__ float taken(const T* x, const uint8_t* ok,
@@ -241,21 +248,111 @@ __device__ __forceinline__ void take_out(float (&f)[N][V], int slot) {
     f[i / V][i % V] = i == slot ? -INFINITY : f[i / V][i % V];
 }
 
-// The key of the at-th logit of lane l, of lanes with every G-th vector.
+// Where in its row the at-th logit of lane l is, of lanes with every G-th
+// vector.
 template <typename T, int G>
-__device__ __forceinline__ uint64_t key_at(float v, int l, int at, int A) {
+__device__ __forceinline__ int place_of(int l, int at, int A) {
   constexpr int V = kVec<T>;
   const int base = (l + G * (at / V)) * V;
-  const int from = A < V || base < A - V ? base : A - V;
-  return v > -INFINITY ? key_of(v, from + at % V) : 0;
+  return (A < V || base < A - V ? base : A - V) + at % V;
+}
+
+// A lower bound of the k-th largest element that few more than k reach: a
+// bisection between the least and the largest of G lanes' H bests each, no
+// element the best of two, by how many of them reach the middle. First the
+// middle of the values is taken; where that does not come near, as with one
+// value far above the others, that of their exponents. Wherever it ends, its
+// lower end holds.
+template <int G, int H>
+__device__ __forceinline__ float bound_of(const float (&heads)[H], float most,
+                                          int k) {
+  const int enough = k + k / 4 + 2;
+  float lo = INFINITY, hi = most;
+#pragma unroll
+  for (int h = 0; h < H; ++h)
+    lo = fminf(lo, heads[h] == -INFINITY ? INFINITY : heads[h]);
+  lo = -group_max<G>(-lo);
+  auto reach = [&](float v) {
+    uint32_t n = 0;
+#pragma unroll
+    for (int h = 0; h < H; ++h) n += heads[h] >= v;
+    return (int)group_reduce<G>(n,
+                                [](uint32_t a, uint32_t b) { return a + b; });
+  };
+  int n = reach(lo);
+  if (n < k) return -3.402823466e38f;
+  for (int i = 0; i < 24 && n > enough && lo < hi; ++i) {
+    float mid = 0.5f * lo + 0.5f * hi;
+    if (i >= 6) {
+      // whole numbers in the order of the values
+      const int a = __float_as_int(lo), b = __float_as_int(hi);
+      const int from = a ^ (a >> 31 & 0x7fffffff);
+      const int to = b ^ (b >> 31 & 0x7fffffff);
+      const int at = from + (int)(((uint32_t)to - (uint32_t)from + 1) / 2);
+      mid = __int_as_float(at ^ (at >> 31 & 0x7fffffff));
+    }
+    const int some = reach(mid);
+    if (some < k) {
+      hi = mid;
+    } else {
+      lo = mid;
+      n = some;
+    }
+  }
+  return lo;
+}
+
+// A wave's writes to LDS are there for its reads behind this.
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// Keys of short rows: 19 bits hold a 16-bit type's values in 32 bits, the
+// other 13 an index below 2^13. 0 is nothing, as for the wide ones.
+template <typename T>
+using Key = std::conditional_t<sizeof(T) == 2, uint32_t, uint64_t>;
+
+template <typename K>
+__device__ __forceinline__ K short_key(float v, int i) {
+  const uint64_t key = key_of(v, i);
+  if constexpr (sizeof(K) == 8) return key;
+  return ((uint32_t)(key >> 32) & ~0x1fffu) | (0x1fffu - (uint32_t)i);
+}
+__device__ __forceinline__ uint64_t wide_key(uint64_t key) { return key; }
+__device__ __forceinline__ uint64_t wide_key(uint32_t key) {
+  const uint32_t low = key & 0x80000000u ? 0 : 0x1fffu;
+  return (uint64_t)((key & ~0x1fffu) | low) << 32 |
+         (0xffffffffu - (0x1fffu - (key & 0x1fffu)));
 }
 
 // ---- rows of up to G * N vectors: G lanes a row, all of it in registers
 // Few lanes with up to four vectors each share a row's bookkeeping among few:
 // 524288 x 17 fp32 takes 17 us with 2 lanes of 3 vectors, 25 with 8 of one.
+// Rows of so many lanes find their alternatives by a bound, 64199 x 886 bf16
+// with 14 in 57 us (in rounds 164). Fewer lanes take a round an alternative:
+// 65536 x 100 bf16 with 5 takes 12.4 us so, by a bound 17.6.
+template <int G>
+constexpr bool kRanked = G >= 8;
+// Keys that a row's lanes rank among themselves: what reaches the bound, of
+// which there are more the closer k comes to 64.
+template <int G>
+constexpr int kCap = G == 64 ? 512 : G == 32 ? 320 : G == 16 ? 192 : 128;
+
 template <typename T, int G, int N, bool TOP>
-__global__ __launch_bounds__(256) void logp_group_kernel(LogpFwd p) {
+__global__ __launch_bounds__(256, TOP && kRanked<G> ? 4 : 1)
+void logp_group_kernel(LogpFwd p) {
   constexpr int V = kVec<T>, R = 256 / G;
+  // 64 bests a row, each of C of a lane's elements
+  constexpr int C = (N * V + kWave / G - 1) / (kWave / G);
+  constexpr int H = (N * V + C - 1) / C;
+  constexpr bool kFind = TOP && kRanked<G>;
+  using K = Key<T>;
+  // zeros behind the last, and no two rows at one bank
+  constexpr int kRow = kFind ? kCap<G> + 80 / sizeof(K) : 1;
+  static_assert(!kFind || kRow >= kCap<G> + kAhead);
+  __shared__ alignas(16) K found[kFind ? R : 1][kRow];
+  __shared__ int counts[kFind ? R : 1];
   const int l = threadIdx.x % G, A = (int)p.A;
   for (int64_t row = (int64_t)blockIdx.x * R + threadIdx.x / G; row < p.rows;
        row += (int64_t)gridDim.x * R) {
@@ -277,6 +374,7 @@ __global__ __launch_bounds__(256) void logp_group_kernel(LogpFwd p) {
       for (int e = 0; e < V; ++e) m = maximum(m, f[i][e]);
     }
     m = group_max<G>(m);
+    const float most = m;
     if (m == -INFINITY) m = 0.f;
     float s = 0.f, u = 0.f;
 #pragma unroll
@@ -291,14 +389,90 @@ __global__ __launch_bounds__(256) void logp_group_kernel(LogpFwd p) {
     u = group_sum<G>(u);
     if (l == 0) finish_row(p, row, act, q, m, s, u);
     if constexpr (!TOP) continue;
-    // a round an alternative; the one found is taken out
-    for (int j = 0; j < p.k; ++j) {
-      int slot;
-      const float top = first_best(f, slot);
-      const uint64_t own = key_at<T, G>(top, l, slot, A);
-      const uint64_t best = group_larger<G>(own);
-      if (own == best) take_out(f, slot);
-      if (l == 0) finish_top(p, row, j, best, m, s);
+    const Top to_row(p, row, m, s);
+    int count = kCap<G> + 1;
+    if constexpr (kRanked<G>) {
+      K* keys = found[threadIdx.x / G];
+      int* at = &counts[threadIdx.x / G];
+      float heads[H];
+#pragma unroll
+      for (int h = 0; h < H; ++h) {
+        heads[h] = -INFINITY;
+#pragma unroll
+        for (int i = h * C; i < (h + 1) * C && i < N * V; ++i)
+          heads[h] = fmaxf(heads[h], f[i / V][i % V]);
+      }
+      const float least =
+          bound_of<G, H>(heads, to_row.broken ? -INFINITY : most, p.k);
+      uint32_t mine = 0;  // a bit for each element that reaches it
+#pragma unroll
+      for (int i = N * V - 1; i >= 0; --i)
+        mine = mine + mine + (f[i / V][i % V] >= least);
+      if (to_row.broken) mine = 0;
+      if (l == 0) *at = 0;
+      wave_sync();
+      int to = mine ? atomicAdd(at, __popc(mine)) : 0;
+      for (; mine; mine &= mine - 1, ++to) {
+        const int j = place_of<T, G>(l, __ffs(mine) - 1, A);
+        if (to < kCap<G>) keys[to] = short_key<K>((float)x[j], j);
+      }
+      wave_sync();
+      count = *at;
+      if (count <= kCap<G>) {
+        for (int i = l; i < kAhead; i += G) keys[count + i] = 0;
+        wave_sync();
+        for (int i = l; i < count; i += G) {
+          const K own = keys[i];
+          int rank = 0;
+          for (int j = 0; j < count; j += 8) {
+            K other[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) other[e] = keys[j + e];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) rank += other[e] > own;
+          }
+          if (rank < p.k) to_row.put(rank, wide_key(own));
+        }
+        for (int i = count + l; i < p.k; i += G) to_row.put(i, 0);
+        wave_sync();
+      }
+    }
+    if (count <= kCap<G>) continue;
+    // a round an alternative
+    if constexpr (sizeof(K) == 4 && !kRanked<G>) {
+      K keys[N * V], last = ~(K)0;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        int from = place_of<T, G>(l, i * V, A);
+        asm volatile("" : "+v"(from));  // its sums are not kept for later rows
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          keys[i * V + e] =
+              f[i][e] > -INFINITY ? short_key<K>(f[i][e], from + e) : 0;
+      }
+      for (int j = 0; j < p.k; ++j) {
+        // Below the last one, differences to it wrap: the largest of all is
+        // the nearest below it.
+        if (last) {
+          K best = 0;
+#pragma unroll
+          for (int i = 0; i < N * V; ++i) best = max(best, keys[i] - last);
+          last += group_reduce<G>(best,
+                                  [](K a, K b) { return a > b ? a : b; });
+        }
+        if (l == 0) to_row.put(j, last ? wide_key(last) : 0);
+      }
+    } else {
+      // the one found is taken out
+      for (int j = 0; j < p.k; ++j) {
+        int slot;
+        const float top = first_best(f, slot);
+        const uint64_t own =
+            top > -INFINITY ? key_of(top, place_of<T, G>(l, slot, A)) : 0;
+        const uint64_t best = group_larger<G>(own);
+        if (own == best) take_out(f, slot);
+        if (l == 0) to_row.put(j, best);
+      }
     }
   }
 }
@@ -464,9 +638,10 @@ __global__ __launch_bounds__(kLanes) void logp_row_kernel(LogpFwd p,
       }
     }
     if (TOP) {
+      const Top to_row(p, row, m, s);
       auto put = [&](int i, uint64_t key) {
         if (P == 1) {
-          finish_top(p, row, i, key, m, s);
+          to_row.put(i, key);
         } else {
           parts.keys[b * p.k + i] = key;
         }
@@ -536,7 +711,7 @@ __global__ __launch_bounds__(kLanes) void logp_row_kernel(LogpFwd p,
 // lane's registers: nothing is read twice.
 constexpr int kHeld = 2 * kLanes;
 
-template <typename T, int N>
+template <typename T, int N = kHeld / kLanes>
 __global__ __launch_bounds__(kLanes) void logp_part_kernel(LogpFwd p,
                                                            Parts parts) {
   constexpr int V = kVec<T>, W = kLanes / kWave;
@@ -615,9 +790,10 @@ __global__ __launch_bounds__(kLanes) void logp_part_kernel(LogpFwd p,
         parts.sums[3 * b + 2] = u;
       }
     }
+    const Top to_row(p, row, m, s);
     auto put = [&](int i, uint64_t key) {
       if (P == 1) {
-        finish_top(p, row, i, key, m, s);
+        to_row.put(i, key);
       } else {
         parts.keys[b * p.k + i] = key;
       }
@@ -694,6 +870,7 @@ __global__ __launch_bounds__(kLanes) void logp_join_kernel(LogpFwd p,
     }
     if (k == 0) continue;
     const uint64_t* keys = parts.keys + row * P * k;
+    const Top to_row(p, row, r.m, r.s);
     const int each = (k + P - 1) / P, n = P * each;  // < k + P
     if (tid < n) heads[tid] = keys[tid / each * k + tid % each];
     __syncthreads();
@@ -707,10 +884,9 @@ __global__ __launch_bounds__(kLanes) void logp_join_kernel(LogpFwd p,
     for (int i = tid; i < count; i += kLanes) {
       const uint64_t mine = found[i];
       const int rank = rank_of(mine, found, count);
-      if (rank < k) finish_top(p, row, rank, mine, r.m, r.s);
+      if (rank < k) to_row.put(rank, mine);
     }
-    for (int i = count + tid; i < k; i += kLanes)
-      finish_top(p, row, i, 0, r.m, r.s);
+    for (int i = count + tid; i < k; i += kLanes) to_row.put(i, 0);
     __syncthreads();
   }
 }
@@ -761,10 +937,9 @@ Group group_of(int64_t A, int V) {
 }
 
 // Vectors of the longest row that a wave's lanes hold: 8192 x 1000 bf16 takes
-// 6.3 us so, 12.6 in a block a row; 8192 x 2048 10.4 and 15.2. With
-// alternatives, which cost a group a round each, half as many: 8192 x 2048
-// with 20 takes 66 us in rounds, 33 in blocks. Longer ones take blocks.
-constexpr int64_t group_vecs(int k) { return k ? 2 * kWave : 4 * kWave; }
+// 6.3 us so, 12.6 in a block a row; 8192 x 2048 10.4 and 15.2, with 20
+// alternatives 17 and 32. Longer ones take blocks.
+constexpr int64_t kGroupVecs = 4 * kWave;
 
 template <typename T, bool BWD, int G, int N, typename P>
 hipError_t group_with(const P& p, hipStream_t s) {
@@ -774,11 +949,8 @@ hipError_t group_with(const P& p, hipStream_t s) {
   if constexpr (BWD) {
     return launch(logp_group_bwd_kernel<T, G, N>, grid, dim3(B), 0, s, p);
   } else {
-    if constexpr (G < kWave) {
-      if (p.k)
-        return launch(logp_group_kernel<T, G, N, true>, grid, dim3(B), 0, s,
-                      p);
-    }
+    if (p.k)
+      return launch(logp_group_kernel<T, G, N, true>, grid, dim3(B), 0, s, p);
     return launch(logp_group_kernel<T, G, N, false>, grid, dim3(B), 0, s, p);
   }
 }
@@ -809,16 +981,17 @@ hipError_t group(const P& p, hipStream_t s) {
 
 // Parts of a row: of 512 vectors at least, while there are fewer blocks than
 // keep the chip busy (97 x 100000 bf16: 10 us in parts, 20 whole; 512 x 32768:
-// 13 and 10); with alternatives of as many as registers hold at most, which
-// are then read once.
+// 13 and 10); with alternatives of as many as registers hold, which are then
+// read once.
 constexpr int64_t kBlocks = 512;
 
 int parts_of(int64_t rows, int64_t A, int k, int V) {
   const int64_t n = (A + V - 1) / V;
-  if (n <= group_vecs(k) || rows <= 0) return 1;
-  int64_t p = (kBlocks + rows - 1) / rows;
-  p = p < n / 512 ? p : n / 512;
-  if (k && p < (n + kHeld - 1) / kHeld) p = (n + kHeld - 1) / kHeld;
+  if (n <= kGroupVecs || rows <= 0) return 1;
+  const int64_t want = (kBlocks + rows - 1) / rows;
+  int64_t p = k               ? (n + kHeld - 1) / kHeld
+              : want < n / 512 ? want
+                               : n / 512;
   p = p < kMostParts ? p : kMostParts;
   return p < 1 ? 1 : (int)p;
 }
@@ -827,7 +1000,7 @@ template <typename T>
 hipError_t fwd(const LogpFwd& p, void* scratch, int type, hipStream_t s) {
   if (p.rows == 0) return hipSuccess;
   const int64_t n = (p.A + kVec<T> - 1) / kVec<T>;
-  if (n <= group_vecs(p.k)) return group<T, false>(p, s);
+  if (n <= kGroupVecs) return group<T, false>(p, s);
   const int P = parts_of(p.rows, p.A, p.k, kVec<T>);
   const int64_t blocks = p.rows * P;
   const Parts parts = {(float*)((uint64_t*)scratch + blocks * p.k),
@@ -837,11 +1010,8 @@ hipError_t fwd(const LogpFwd& p, void* scratch, int type, hipStream_t s) {
   hipError_t e;
   if (p.k == 0) {
     e = launch(logp_row_kernel<T, false>, grid, lanes, 0, s, p, parts);
-  } else if (n <= (int64_t)kLanes * P) {
-    e = launch(logp_part_kernel<T, 1>, grid, lanes, 0, s, p, parts);
   } else if (n <= (int64_t)kHeld * P) {
-    e = launch(logp_part_kernel<T, kHeld / kLanes>, grid, lanes, 0, s, p,
-               parts);
+    e = launch(logp_part_kernel<T>, grid, lanes, 0, s, p, parts);
   } else {
     e = launch(logp_row_kernel<T, true>, grid, lanes, 0, s, p, parts);
   }
@@ -854,7 +1024,7 @@ template <typename T>
 hipError_t bwd(const LogpBwd& p, hipStream_t s) {
   if (p.rows == 0) return hipSuccess;
   const int64_t n = (p.A + kVec<T> - 1) / kVec<T>;
-  if (n <= group_vecs(0)) return group<T, true>(p, s);
+  if (n <= kGroupVecs) return group<T, true>(p, s);
   const int64_t pieces = (n + 256 * kBwdVecs - 1) / (256 * kBwdVecs);
   const int64_t grid = p.rows * pieces;
   return launch(logp_row_bwd_kernel<T>, dim3(grid < kGrid ? grid : kGrid),

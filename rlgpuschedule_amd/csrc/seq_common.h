@@ -61,7 +61,7 @@ __device__ __forceinline__ float maximum(float a, float b) {
 // other lanes than an exclusive-or's would, but hold the same sums.
 template <int CTRL>
 __device__ __forceinline__ uint32_t dpp(uint32_t v) {
-  return __builtin_amdgcn_update_dpp(v, v, CTRL, 0xf, 0xf, false);
+  return __builtin_amdgcn_update_dpp(0, v, CTRL, 0xf, 0xf, true);
 }
 
 template <int W = kWave, typename Op>

@@ -661,6 +661,32 @@ def test_logp_hard_rows(device, dtype, A):
 
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("A", [70, 130, 257, 500, 777, 1100, 2000])
+@pytest.mark.parametrize("k", [1, 7, 40, 64])
+def test_logp_alternatives(device, dtype, A, k):
+    """Rows in which a bound of the k best is hard to find, or in which many
+    reach it."""
+    g = gen(A * 65 + k)
+    x = randn(g, 11, A, dtype=F32, scale=2.0)
+    mask = torch.ones(11, A, dtype=torch.uint8)
+    x[1] = torch.randint(0, 3, (A,), generator=g)    # three values
+    x[2, A // 2] = 3e4                               # one far above
+    x[3, ::3] = -3e4                                 # some far below
+    mask[4] = torch.rand(A, generator=g) < 0.05      # few allowed
+    x[5] = torch.exp2(torch.randint(-20, 15, (A,), generator=g).float())
+    x[6] = -x[5]
+    x[7] = torch.sort(x[7]).values.flip(0)           # best ones together
+    mask[8] = 0
+    mask[8, A // 3:A // 3 + 40] = 1                  # allowed ones together
+    x[9, A // 2:] = x[9, :A - A // 2].clone()        # each value twice
+    x[10] = 1.0 + torch.arange(A) * 1e-7             # hardly apart
+    act = torch.randint(0, A, (11,), generator=g)
+    check_logp(x.to(dtype).to(device), act.to(device), mask.to(device), k,
+               torch.ones(11, device=device), None, f"{A} {k} {dtype}")
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("A", [19, 120, 5000])
 def test_logp_layouts(device, dtype, A):
     g = gen(A + 1)
