@@ -95,8 +95,9 @@ MaybeTensor maybe(const Tensor& t) {
 }
 // Values as memory holds them: torch notes a conjugate's imaginary part as to
 // be negated.
+Tensor plain(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
 MaybeTensor packed(const MaybeTensor& t) {
-  return t && t->defined() ? MaybeTensor(t->resolve_neg().contiguous())
+  return t && t->defined() ? MaybeTensor(plain(*t).contiguous())
                            : std::nullopt;
 }
 
@@ -108,7 +109,7 @@ Tensor f32(const Tensor& x, at::IntArrayRef size) {
 // next. Leading dims that no single stride walks, and last dims of another
 // stride, are copied.
 std::pair<Tensor, int64_t> rows_of(const Tensor& t_) {
-  const Tensor t = t_.resolve_neg();
+  const Tensor t = plain(t_);
   const int64_t d = t.size(-1);
   if (t.is_contiguous()) return {t, d};
   Tensor r = t.reshape({-1, d});
@@ -118,7 +119,7 @@ std::pair<Tensor, int64_t> rows_of(const Tensor& t_) {
 
 // t [..., E, H] with neighbouring columns and environments within reach.
 Tensor reachable(const Tensor& t_) {
-  const Tensor t = t_.resolve_neg();
+  const Tensor t = plain(t_);
   const bool near = t.stride(-2) <= rlsched_scan_reach(t.size(-1));
   const bool unit = t.size(-1) == 1 || t.stride(-1) == 1;
   return near && unit ? t : t.contiguous();
