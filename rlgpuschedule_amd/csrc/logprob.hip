@@ -217,18 +217,6 @@ __device__ __forceinline__ int rank_of(uint64_t mine, const uint64_t* keys,
   return rank;
 }
 
-// A lower bound of the k-th largest element, from 64 lanes' or groups' bests,
-// no element the best of two: the least that fewer than k are above. At least
-// the lowest finite value. For one wave; the result is in all its lanes.
-__device__ __forceinline__ float least_of(const float* heads, int k) {
-  const float mine = heads[threadIdx.x % kWave];
-  int above = 0;
-#pragma unroll
-  for (int i = 0; i < kWave; ++i) above += heads[i] > mine;
-  const float least = -group_max(above < k ? -mine : -INFINITY);
-  return fmaxf(least, -3.402823466e38f);
-}
-
 // The largest of a lane's logits, and where it is first.
 template <int N, int V>
 __device__ __forceinline__ float first_best(const float (&f)[N][V],
@@ -274,6 +262,11 @@ __device__ __forceinline__ float bound_of(const float (&heads)[H], float most,
   lo = -group_max<G>(-lo);
   auto reach = [&](float v) {
     uint32_t n = 0;
+    if constexpr (G == kWave) {
+#pragma unroll
+      for (int h = 0; h < H; ++h) n += __popcll(__ballot(heads[h] >= v));
+      return (int)n;
+    }
 #pragma unroll
     for (int h = 0; h < H; ++h) n += heads[h] >= v;
     return (int)group_reduce<G>(n,
@@ -334,17 +327,20 @@ __device__ __forceinline__ uint64_t wide_key(uint32_t key) {
 // 65536 x 100 bf16 with 5 takes 12.4 us so, by a bound 17.6.
 template <int G>
 constexpr bool kRanked = G >= 8;
+// Bests of a row that its bound is found from: of 64, 8192 x 2048 bf16 with 64
+// alternatives takes 119 us instead of 29, and 17 with 20 alternatives as well.
+constexpr int kBests = 128;
 // Keys that a row's lanes rank among themselves: what reaches the bound, of
-// which there are more the closer k comes to 64.
+// 128 bests' 82 about 130.
 template <int G>
-constexpr int kCap = G == 64 ? 512 : G == 32 ? 320 : G == 16 ? 192 : 128;
+constexpr int kCap = G >= 32 ? 256 : G == 16 ? 192 : 128;
 
 template <typename T, int G, int N, bool TOP>
-__global__ __launch_bounds__(256, TOP && kRanked<G> ? 4 : 1)
+__global__ __launch_bounds__(256, TOP && kRanked<G> && N <= 4 ? 4 : 1)
 void logp_group_kernel(LogpFwd p) {
   constexpr int V = kVec<T>, R = 256 / G;
-  // 64 bests a row, each of C of a lane's elements
-  constexpr int C = (N * V + kWave / G - 1) / (kWave / G);
+  // a row's bests, each of C of a lane's elements
+  constexpr int C = (N * V + kBests / G - 1) / (kBests / G);
   constexpr int H = (N * V + C - 1) / C;
   constexpr bool kFind = TOP && kRanked<G>;
   using K = Key<T>;
@@ -404,16 +400,17 @@ void logp_group_kernel(LogpFwd p) {
       }
       const float least =
           bound_of<G, H>(heads, to_row.broken ? -INFINITY : most, p.k);
-      uint32_t mine = 0;  // a bit for each element that reaches it
+      // a bit for each element that reaches it
+      std::conditional_t<(N * V > 32), uint64_t, uint32_t> mine = 0;
 #pragma unroll
       for (int i = N * V - 1; i >= 0; --i)
         mine = mine + mine + (f[i / V][i % V] >= least);
       if (to_row.broken) mine = 0;
       if (l == 0) *at = 0;
       wave_sync();
-      int to = mine ? atomicAdd(at, __popc(mine)) : 0;
+      int to = mine ? atomicAdd(at, __popcll(mine)) : 0;
       for (; mine; mine &= mine - 1, ++to) {
-        const int j = place_of<T, G>(l, __ffs(mine) - 1, A);
+        const int j = place_of<T, G>(l, __builtin_ctzll(mine), A);
         if (to < kCap<G>) keys[to] = short_key<K>((float)x[j], j);
       }
       wave_sync();
@@ -534,18 +531,24 @@ struct Running {
 };
 
 constexpr int kLanes = 256;
-// Elements that are ranked at once: of 64 bests' least about 300 are above.
+// Elements that are ranked at once.
 constexpr int kFound = 512;
 
-// least_of a block's lanes, four of which have a head. `count` is cleared.
-__device__ __forceinline__ float block_least(float own, int k, float* heads,
+// bound_of a block's lanes. `count` is cleared.
+__device__ __forceinline__ float block_bound(float own, int k, float* heads,
                                              float* at, int* count) {
-  const float head = group_max<4>(own);
-  if (threadIdx.x % 4 == 0) heads[threadIdx.x / 4] = head;
+  heads[threadIdx.x] = own;
   __syncthreads();
   if (threadIdx.x < kWave) {
-    const float least = least_of(heads, k);
-    if (threadIdx.x == 0) *at = least, *count = 0;
+    constexpr int H = kLanes / kWave;
+    float mine[H], most = -INFINITY;
+#pragma unroll
+    for (int h = 0; h < H; ++h) {
+      mine[h] = heads[threadIdx.x + h * kWave];
+      most = maximum(most, mine[h]);
+    }
+    const float bound = bound_of<kWave, H>(mine, group_max(most), k);
+    if (threadIdx.x == 0) *at = bound, *count = 0;
   }
   __syncthreads();
   return *at;
@@ -574,7 +577,7 @@ template <typename T, bool TOP>
 __global__ __launch_bounds__(kLanes) void logp_row_kernel(LogpFwd p,
                                                           Parts parts) {
   constexpr int V = kVec<T>, W = kLanes / kWave, U = 4;
-  __shared__ float sums[3][W], heads[kWave], least_at;
+  __shared__ float sums[3][W], heads[kLanes], least_at;
   __shared__ uint64_t found[kFound + kAhead], waves[W];
   __shared__ int count_at;
   const int tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave;
@@ -648,7 +651,7 @@ __global__ __launch_bounds__(kLanes) void logp_row_kernel(LogpFwd p,
       };
       // only lanes whose own best reaches the bound have more to give
       const float least =
-          block_least(own, p.k, heads, &least_at, &count_at);
+          block_bound(own, p.k, heads, &least_at, &count_at);
       if (own >= least) {
         for (int i = first + tid; i < n; i += U * kLanes) {
           Piece<T> v[U];
@@ -715,7 +718,7 @@ template <typename T, int N = kHeld / kLanes>
 __global__ __launch_bounds__(kLanes) void logp_part_kernel(LogpFwd p,
                                                            Parts parts) {
   constexpr int V = kVec<T>, W = kLanes / kWave;
-  __shared__ float sums[3][W], heads[kWave], least_at;
+  __shared__ float sums[3][W], heads[kLanes], least_at;
   __shared__ uint64_t found[kFound + kAhead], waves[W];
   __shared__ int count_at;
   const int tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave;
@@ -746,7 +749,7 @@ __global__ __launch_bounds__(kLanes) void logp_part_kernel(LogpFwd p,
     float m = group_max(top);
     if (lane == 0) sums[0][wave] = m;
     const float least =
-        block_least(top, p.k, heads, &least_at, &count_at);
+        block_bound(top, p.k, heads, &least_at, &count_at);
 #pragma unroll
     for (int i = 0; i < W; ++i) m = maximum(m, sums[0][i]);
     if (m == -INFINITY) m = -3.402823466e38f;
@@ -924,7 +927,8 @@ __global__ __launch_bounds__(256) void logp_row_bwd_kernel(LogpBwd p,
 
 constexpr int64_t kGrid = 1 << 22;  // blocks at most; more are looped over
 
-// Rows that G lanes hold in registers: G as few as four vectors a lane allow.
+// Rows that G lanes hold in registers: G as few as four vectors a lane allow,
+// and a wave with 6 or 8.
 struct Group {
   int G, N;
 };
@@ -932,14 +936,23 @@ struct Group {
 Group group_of(int64_t A, int V) {
   const int64_t n = (A + V - 1) / V;
   int G = 1;
-  while (4 * G < n) G *= 2;
-  return {G, (int)((n + G - 1) / G)};
+  while (4 * G < n && G < kWave) G *= 2;
+  const int N = (int)((n + G - 1) / G);
+  return {G, N <= 4 ? N : (N + 1) / 2 * 2};
 }
 
-// Vectors of the longest row that a wave's lanes hold: 8192 x 1000 bf16 takes
-// 6.3 us so, 12.6 in a block a row; 8192 x 2048 10.4 and 15.2, with 20
-// alternatives 17 and 32. Longer ones take blocks.
+// Vectors of the longest row that a wave's lanes hold, as many a lane as
+// leave registers for three waves or more; longer ones take blocks. 4 forward
+// and backward: 8192 x 1000 bf16 takes 6.3 us so, 12.6 in blocks, 8192 x 2048
+// 10.4 and 15.2. Forward, 32 bits go to 6: 8192 x 1400 12.4 and 15.5 us (to 8:
+// 8192 x 2048 18.3 and 16.3). With alternatives, which a block finds between
+// barriers, 16 bits go to 6 and 32 to 8: 13938 x 2780 fp16 with 6 takes 37 and
+// 51 us, 8192 x 2048 fp32 with 20 25 and 33 (16 bits to 8: 8192 x 4096 with 20
+// 38 and 37).
 constexpr int64_t kGroupVecs = 4 * kWave;
+constexpr int64_t group_vecs(int k, int V) {
+  return (V == 4 ? k ? 8 : 6 : k ? 6 : 4) * kWave;
+}
 
 template <typename T, bool BWD, int G, int N, typename P>
 hipError_t group_with(const P& p, hipStream_t s) {
@@ -958,6 +971,10 @@ hipError_t group_with(const P& p, hipStream_t s) {
 template <typename T, bool BWD, typename P>
 hipError_t group(const P& p, hipStream_t s) {
   const Group g = group_of(p.A, kVec<T>);
+  if constexpr (!BWD) {
+    if (g.N == 6) return group_with<T, false, 64, 6>(p, s);
+    if (g.N == 8) return group_with<T, false, 64, 8>(p, s);
+  }
   switch (g.G * 8 + g.N) {
     case 1 * 8 + 1: return group_with<T, BWD, 1, 1>(p, s);
     case 1 * 8 + 2: return group_with<T, BWD, 1, 2>(p, s);
@@ -987,7 +1004,7 @@ constexpr int64_t kBlocks = 512;
 
 int parts_of(int64_t rows, int64_t A, int k, int V) {
   const int64_t n = (A + V - 1) / V;
-  if (n <= kGroupVecs || rows <= 0) return 1;
+  if (n <= group_vecs(k, V) || rows <= 0) return 1;
   const int64_t want = (kBlocks + rows - 1) / rows;
   int64_t p = k               ? (n + kHeld - 1) / kHeld
               : want < n / 512 ? want
@@ -1000,7 +1017,7 @@ template <typename T>
 hipError_t fwd(const LogpFwd& p, void* scratch, int type, hipStream_t s) {
   if (p.rows == 0) return hipSuccess;
   const int64_t n = (p.A + kVec<T> - 1) / kVec<T>;
-  if (n <= kGroupVecs) return group<T, false>(p, s);
+  if (n <= group_vecs(p.k, kVec<T>)) return group<T, false>(p, s);
   const int P = parts_of(p.rows, p.A, p.k, kVec<T>);
   const int64_t blocks = p.rows * P;
   const Parts parts = {(float*)((uint64_t*)scratch + blocks * p.k),
