@@ -579,7 +579,7 @@ __global__ __launch_bounds__(kLanes) void logp_row_kernel(LogpFwd p,
   constexpr int V = kVec<T>, W = kLanes / kWave, U = 4;
   __shared__ float sums[3][W], heads[kLanes], least_at;
   __shared__ uint64_t found[kFound + kAhead], waves[W];
-  __shared__ int count_at;
+  __shared__ int count_at, hot_at, hot[kLanes];
   const int tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave;
   const int A = (int)p.A, all = (A + V - 1) / V, P = parts.parts;
   for (int64_t b = blockIdx.x; b < p.rows * P; b += gridDim.x) {
@@ -649,26 +649,34 @@ __global__ __launch_bounds__(kLanes) void logp_row_kernel(LogpFwd p,
           parts.keys[b * p.k + i] = key;
         }
       };
-      // only lanes whose own best reaches the bound have more to give
+      if (tid == 0) hot_at = 0;
       const float least =
           block_bound(own, p.k, heads, &least_at, &count_at);
-      if (own >= least) {
-        for (int i = first + tid; i < n; i += U * kLanes) {
-          Piece<T> v[U];
+      // Only the vectors of lanes whose own best reaches the bound have more to
+      // give: they are read again, by all lanes.
+      if (own >= least) hot[atomicAdd(&hot_at, 1)] = tid;
+      __syncthreads();
+      const int each = (n - first + kLanes - 1) / kLanes, some = hot_at * each;
+      for (int i = tid; i < some; i += 2 * kLanes) {
+        Piece<T> v[2];
+        bool in[2];
 #pragma unroll
-          for (int c = 0; c < U; ++c)
-            if (i + c * kLanes < n) v[c].read(x, ok, A, i + c * kLanes);
+        for (int c = 0; c < 2; ++c) {
+          const int at = i + c * kLanes, h = at / each;
+          const int j = at < some ? first + hot[h] + (at - h * each) * kLanes : n;
+          in[c] = j < n;
+          if (in[c]) v[c].read(x, ok, A, j);
+        }
 #pragma unroll
-          for (int c = 0; c < U; ++c) {
-            if (i + c * kLanes >= n) continue;
-            float f[V];
-            v[c].values(ok, f);
+        for (int c = 0; c < 2; ++c) {
+          if (!in[c]) continue;
+          float f[V];
+          v[c].values(ok, f);
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-              if (!(f[e] >= least)) continue;
-              const int at = atomicAdd(&count_at, 1);
-              if (at < kFound) found[at] = key_of(f[e], v[c].from + e);
-            }
+          for (int e = 0; e < V; ++e) {
+            if (!(f[e] >= least)) continue;
+            const int at = atomicAdd(&count_at, 1);
+            if (at < kFound) found[at] = key_of(f[e], v[c].from + e);
           }
         }
       }
@@ -710,11 +718,10 @@ __global__ __launch_bounds__(kLanes) void logp_row_kernel(LogpFwd p,
   }
 }
 
-// The same for parts of up to kHeld vectors with alternatives, N of them in a
-// lane's registers: nothing is read twice.
-constexpr int kHeld = 2 * kLanes;
-
-template <typename T, int N = kHeld / kLanes>
+// The same for parts of up to N * kLanes vectors with alternatives, N of them
+// in a lane's registers: nothing is read twice, 30000 x 4500 bf16 with 20 takes
+// 168 us so and 212 walked, 8192 x 4096 38 and 70.
+template <typename T, int N>
 __global__ __launch_bounds__(kLanes) void logp_part_kernel(LogpFwd p,
                                                            Parts parts) {
   constexpr int V = kVec<T>, W = kLanes / kWave;
@@ -998,17 +1005,15 @@ hipError_t group(const P& p, hipStream_t s) {
 
 // Parts of a row: of 512 vectors at least, while there are fewer blocks than
 // keep the chip busy (97 x 100000 bf16: 10 us in parts, 20 whole; 512 x 32768:
-// 13 and 10); with alternatives of as many as registers hold, which are then
-// read once.
+// 13 and 10). With alternatives too: cut into as many parts as registers hold,
+// 4096 x 32768 bf16 with 8 took 131 us, walked whole 71.
 constexpr int64_t kBlocks = 512;
 
 int parts_of(int64_t rows, int64_t A, int k, int V) {
   const int64_t n = (A + V - 1) / V;
   if (n <= group_vecs(k, V) || rows <= 0) return 1;
-  const int64_t want = (kBlocks + rows - 1) / rows;
-  int64_t p = k               ? (n + kHeld - 1) / kHeld
-              : want < n / 512 ? want
-                               : n / 512;
+  int64_t p = (kBlocks + rows - 1) / rows;
+  p = p < n / 512 ? p : n / 512;
   p = p < kMostParts ? p : kMostParts;
   return p < 1 ? 1 : (int)p;
 }
@@ -1027,8 +1032,12 @@ hipError_t fwd(const LogpFwd& p, void* scratch, int type, hipStream_t s) {
   hipError_t e;
   if (p.k == 0) {
     e = launch(logp_row_kernel<T, false>, grid, lanes, 0, s, p, parts);
-  } else if (n <= (int64_t)kHeld * P) {
-    e = launch(logp_part_kernel<T>, grid, lanes, 0, s, p, parts);
+  } else if (n <= 2 * (int64_t)kLanes * P) {
+    e = launch(logp_part_kernel<T, 2>, grid, lanes, 0, s, p, parts);
+  } else if (n <= 3 * (int64_t)kLanes * P) {
+    e = launch(logp_part_kernel<T, 3>, grid, lanes, 0, s, p, parts);
+  } else if (n <= 4 * (int64_t)kLanes * P) {
+    e = launch(logp_part_kernel<T, 4>, grid, lanes, 0, s, p, parts);
   } else {
     e = launch(logp_row_kernel<T, true>, grid, lanes, 0, s, p, parts);
   }

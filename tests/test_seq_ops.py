@@ -662,7 +662,7 @@ def test_logp_hard_rows(device, dtype, A):
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("A", [70, 130, 257, 500, 777, 1100, 2000,
-                               2800, 4000, 20000])
+                               2800, 4000, 7000, 20000, 300000])
 @pytest.mark.parametrize("k", [1, 7, 40, 64])
 def test_logp_alternatives(device, dtype, A, k):
     """Rows in which a bound of the k best is hard to find, or in which many
