@@ -1006,12 +1006,15 @@ hipError_t group(const P& p, hipStream_t s) {
 // Parts of a row: of 512 vectors at least, while there are fewer blocks than
 // keep the chip busy (97 x 100000 bf16: 10 us in parts, 20 whole; 512 x 32768:
 // 13 and 10). With alternatives too: cut into as many parts as registers hold,
-// 4096 x 32768 bf16 with 8 took 131 us, walked whole 71.
+// 4096 x 32768 bf16 with 8 took 131 us, walked whole 71. Rows of up to kWhole
+// vectors are not cut, which would take a second launch: 16 x 16384 bf16 with
+// 10 takes 8.3 us whole and 9.8 in parts, 16 x 24000 10.8 and 10.6.
+constexpr int64_t kWhole = 2048;
 constexpr int64_t kBlocks = 512;
 
 int parts_of(int64_t rows, int64_t A, int k, int V) {
   const int64_t n = (A + V - 1) / V;
-  if (n <= group_vecs(k, V) || rows <= 0) return 1;
+  if (n <= kWhole || rows <= 0) return 1;
   int64_t p = (kBlocks + rows - 1) / rows;
   p = p < n / 512 ? p : n / 512;
   p = p < kMostParts ? p : kMostParts;
