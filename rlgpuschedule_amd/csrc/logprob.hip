@@ -322,9 +322,10 @@ __device__ __forceinline__ uint64_t wide_key(uint32_t key) {
 // ---- rows of up to G * N vectors: G lanes a row, all of it in registers
 // Few lanes with up to four vectors each share a row's bookkeeping among few:
 // 524288 x 17 fp32 takes 17 us with 2 lanes of 3 vectors, 25 with 8 of one.
-// Rows of so many lanes find their alternatives by a bound, 64199 x 886 bf16
-// with 14 in 57 us (in rounds 164). Fewer lanes take a round an alternative:
-// 65536 x 100 bf16 with 5 takes 12.4 us so, by a bound 17.6.
+
+// So many lanes or more find a row's alternatives by a bound: 64199 x 886 bf16
+// with 14 takes 57 us so, in rounds 164. Fewer take a round an alternative:
+// 1582 x 51 fp32 with 20 takes 11.4 us so, by a bound 17.8.
 template <int G>
 constexpr bool kRanked = G >= 8;
 // Bests of a row that its bound is found from: of 64, 8192 x 2048 bf16 with 64

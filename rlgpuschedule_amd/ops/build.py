@@ -1,7 +1,7 @@
 """In-tree hipcc build of the CDNA4 extensions (gfx950 only, no JIT cache).
 
-Built .so files live next to this file so they travel with the repo snapshot
-to GPU boxes (they are git-ignored but NOT gpurun-ignored).
+Built .so files live next to this file (git-ignored), so that a copy of the
+tree carries them to machines that do not build.
 """
 from __future__ import annotations
 
