@@ -301,9 +301,11 @@ __global__ __launch_bounds__(256) void scan_fwd_way_kernel(ScanFwd p,
   keep_way<V>(p.c, l, w, ways);
 }
 
-// ---- from chunk to chunk, in either direction: 64 columns a block, its 16
-// waves one after the other in time, kJoin chunks each
-constexpr int kJoin = 16;
+// ---- from chunk to chunk, in either direction: kCols columns a block, its
+// kGroups groups of as many lanes one after the other in time, JOIN chunks
+// each. With 64 columns a block few have work: 32768x1x256 fp32's 2048 chunks
+// took 37 us to join, 22 so.
+constexpr int kCols = 32, kGroups = 1024 / kCols;
 
 struct Join {
   const float* ways;   // [chunks, 2, EH]
@@ -313,19 +315,20 @@ struct Join {
   bool reverse;
 };
 
+template <int JOIN>
 __global__ __launch_bounds__(1024) void scan_join_kernel(Join p) {
-  __shared__ float lds[2][16][2][kWave];
-  const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
-  const int64_t col = (int64_t)blockIdx.x * kWave + lane;
+  __shared__ float lds[2][kGroups][2][kCols];
+  const int group = threadIdx.x / kCols, lane = threadIdx.x % kCols;
+  const int64_t col = (int64_t)blockIdx.x * kCols + lane;
   const bool mine = col < p.EH;
   float c = mine && p.first ? p.first[col] : 0.f;
   int turn = 0;
-  for (int64_t k0 = 0; k0 < p.chunks; k0 += 16 * kJoin, turn ^= 1) {
-    const int64_t k = k0 + wave * kJoin;
-    float A[kJoin], B[kJoin];
+  for (int64_t k0 = 0; k0 < p.chunks; k0 += kGroups * JOIN, turn ^= 1) {
+    const int64_t k = k0 + group * JOIN;
+    float A[JOIN], B[JOIN];
     Way w;
 #pragma unroll
-    for (int i = 0; i < kJoin; ++i) {
+    for (int i = 0; i < JOIN; ++i) {
       A[i] = 1.f;
       B[i] = 0.f;
       if (k + i < p.chunks && mine) {
@@ -335,20 +338,20 @@ __global__ __launch_bounds__(1024) void scan_join_kernel(Join p) {
       }
     }
 #pragma unroll
-    for (int i = 0; i < kJoin; ++i) w.then(A[i], B[i]);
-    lds[turn][wave][0][lane] = w.A;
-    lds[turn][wave][1][lane] = w.B;
+    for (int i = 0; i < JOIN; ++i) w.then(A[i], B[i]);
+    lds[turn][group][0][lane] = w.A;
+    lds[turn][group][1][lane] = w.B;
     // one barrier a turn: the next turn writes the other half
     __syncthreads();
     float start = c;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      if (i == wave) start = c;
+    for (int i = 0; i < kGroups; ++i) {
+      if (i == group) start = c;
       const float a = lds[turn][i][0][lane], b = lds[turn][i][1][lane];
       c = a < 0.f ? b : a * c + b;
     }
 #pragma unroll
-    for (int i = 0; i < kJoin; ++i) {
+    for (int i = 0; i < JOIN; ++i) {
       if (k + i < p.chunks && mine) {
         const int64_t at = p.reverse ? p.chunks - 1 - (k + i) : k + i;
         p.carry[at * p.EH + col] = start;
@@ -629,9 +632,11 @@ Plan plan(int64_t T, int64_t E, int64_t H, int bytes, bool back) {
 }
 
 // A chunk follows the ways of up to kFollow others itself, without a kernel
-// between: 509x37x263 fp16's 22 chunks are walked 4 us sooner each way. More
-// would read too much: scratch then holds the chunks' starts as well.
-constexpr int64_t kFollow = 32;
+// between: 509x37x263 fp16's 22 chunks are walked 4 us sooner each way,
+// 663x36x64 bf16's 42 0.3 and 0.9 us, and a launch is saved. More would read
+// too much (2063x3x64 fp32's 129: 20 us instead of 12.5): scratch then holds
+// the chunks' starts as well.
+constexpr int64_t kFollow = 64;
 
 template <typename P>
 void give_ways(P& p, const Plan& q, float* scratch) {
@@ -645,8 +650,12 @@ void give_ways(P& p, const Plan& q, float* scratch) {
 hipError_t join(const float* ways, const float* first, float* carry,
                 const Plan& q, int64_t EH, bool reverse, hipStream_t s) {
   const Join j = {ways, first, carry, EH, q.chunks, reverse};
-  return launch(scan_join_kernel, dim3((EH + kWave - 1) / kWave), dim3(1024),
-                0, s, j);
+  const dim3 grid((EH + kCols - 1) / kCols), block(1024);
+  // fewer chunks a group where one turn is enough: 1473x1x181 bf16 runs in
+  // 10.6 us so and in 11.4 with 16; 7065x11x64's 295 in 24.2 and 23.1
+  if (q.chunks <= 8 * kGroups)
+    return launch(scan_join_kernel<8>, grid, block, 0, s, j);
+  return launch(scan_join_kernel<16>, grid, block, 0, s, j);
 }
 
 template <typename T, int V, bool DONE>

@@ -312,7 +312,8 @@ def run_scan(gate, x, h0, done, dhs, dhl):
 SCAN_SIZES = [(1, 1, 1), (1, 5, 64), (2, 3, 7), (5, 2, 130), (16, 4, 64),
               (17, 3, 72), (63, 2, 33), (64, 3, 256), (65, 2, 64),
               (100, 1, 1000), (129, 5, 40), (256, 1, 8), (300, 2, 66),
-              (1025, 1, 64), (2500, 1, 3), (4100, 2, 20)]
+              (1025, 1, 64), (2500, 1, 3), (4100, 2, 20), (700, 2, 30),
+              (9000, 1, 5)]
 
 
 @pytest.mark.parametrize("device", DEVICES)
