@@ -21,7 +21,7 @@
 // (217 MB with the kept states, 4.7 TB/s) and 70 us backward (352 MB, 5.0), a
 // large copy's rate being 4.9. In chunks gate and x are read twice: 32768 x 2
 // x 1000 takes 70 us for the effects (262 MB; reading alone runs at 4.0 TB/s),
-// 12 to join 512 chunks and 64 to walk. Small calls are bound by the latency
+// 8 to join 512 chunks and 64 to walk. Small calls are bound by the latency
 // of kKeep steps after another: 65 x 64 x 256 bf16 takes 7.5 and 11 us.
 #include "seq_api.h"
 #include "seq_common.h"
