@@ -405,26 +405,34 @@ template <typename W>
 __global__ __launch_bounds__(32 * kSumLanes) void norm_sum_kernel(NormSum a) {
   __shared__ float lds[kSumLanes][32];
   const int lane = threadIdx.x % 32, part = threadIdx.x / 32;
-  const int64_t c = (int64_t)blockIdx.x * 32 + lane;  // of 2 D
-  float v = 0.f;
-  if (c < 2 * a.dim) {
+  for (int64_t c0 = (int64_t)blockIdx.x * 32; c0 < 2 * a.dim;
+       c0 += (int64_t)gridDim.x * 32) {
+    const int64_t c = c0 + lane;  // of 2 D
+    const bool in = c < 2 * a.dim;
+    float v = 0.f;
+    if (in) {
 #pragma unroll 8
-    for (int k = part; k < a.parts; k += kSumLanes)
-      v += a.partial[2 * k * a.dim + c];
-  }
-  lds[part][lane] = v;
-  __syncthreads();
-  if (part || c >= 2 * a.dim) return;
+      for (int k = part; k < a.parts; k += kSumLanes)
+        v += a.partial[2 * k * a.dim + c];
+    }
+    lds[part][lane] = v;
+    __syncthreads();
+    if (part == 0 && in) {
 #pragma unroll
-  for (int k = 1; k < kSumLanes; ++k) v += lds[k][lane];
-  if (c < a.dim) {
-    if (a.dw) ((W*)a.dw)[c] = (W)v;
-  } else {
-    if (a.db) ((W*)a.db)[c - a.dim] = (W)v;
+      for (int k = 1; k < kSumLanes; ++k) v += lds[k][lane];
+      if (c < a.dim) {
+        if (a.dw) ((W*)a.dw)[c] = (W)v;
+      } else {
+        if (a.db) ((W*)a.db)[c - a.dim] = (W)v;
+      }
+    }
+    __syncthreads();  // the next turn writes what this one reads
   }
 }
 
-constexpr int64_t kGrid = 1 << 22;  // blocks at most; more rows are looped over
+// Blocks of 1024 lanes at most, of which a launch has fewer than 2^32; more
+// rows or columns are looped over.
+constexpr int64_t kGrid = 1 << 21;
 
 // How a row lies on lanes: G of them with N vectors each; G = 0: too long.
 // Two vectors a lane, for twice the bytes in flight: with one, 131072 x 256
@@ -517,7 +525,8 @@ hipError_t bwd(const NormBwd& p, const NormSum& z, hipStream_t s) {
                    dim3((p.dim + 255) / 256, p.parts), dim3(256), 0, s, p);
   }
   if (e != hipSuccess || !p.partial) return e;
-  const dim3 grid((2 * p.dim + 31) / 32);
+  const int64_t sums = (2 * p.dim + 31) / 32;
+  const dim3 grid(sums < kGrid ? sums : kGrid);
   if (p.w32) return launch(norm_sum_kernel<float>, grid, dim3(32 * kSumLanes), 0, s, z);
   return launch(norm_sum_kernel<T>, grid, dim3(32 * kSumLanes), 0, s, z);
 }

@@ -151,12 +151,17 @@ struct OnDevice {
 };
 
 // The launch's own status: an error left by other code stays where it is.
+// 2^32 lanes or more along one axis are refused here: the runtime refuses
+// 2^32 itself, but a launch of 2^32 + 3072 left most of its work undone
+// without an error.
 template <typename... P, typename... A>
 inline hipError_t launch(void (*kernel)(P...), dim3 grid, dim3 block,
                          size_t lds, hipStream_t stream, A... args) {
   void* list[] = {(void*)&args...};
   static_assert(std::is_same_v<std::tuple<P...>, std::tuple<A...>>,
                 "a value of its own type for each parameter");
+  if (((uint64_t)grid.x * block.x | (uint64_t)grid.y * block.y) >> 32)
+    return hipErrorInvalidConfiguration;
   return hipLaunchKernel((const void*)kernel, grid, block, list, lds, stream);
 }
 
