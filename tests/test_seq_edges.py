@@ -5,10 +5,11 @@ import math
 import pytest
 import torch
 
-from rlgpuschedule_amd import layer_norm
+from rlgpuschedule_amd import gated_scan, gated_scan_step, layer_norm
 from rlgpuschedule_amd.ops.norm import layer_norm_bwd, layer_norm_fwd
 
-from test_seq_ops import U, gen, randn
+from test_seq_ops import (DEVICES, U, close, gen, randn, run_scan,
+                          scan_64)
 
 
 # ------------------------------------------------------ launches of 2^32 lanes
@@ -66,3 +67,64 @@ def test_norm_of_2_22_long_rows():
     assert torch.equal(dx[some], dx1.expand(len(some), d))
     del dx
     torch.cuda.empty_cache()
+
+
+# ------------------------------------------------------------ far gates
+def far_gates(g, shape, device):
+    """Gates of magnitudes from 1/2 to 80, of both signs, where one of z and
+    1 - z is down to 1e-35 and still has all its bits."""
+    size = torch.exp2(torch.rand(*shape, generator=g) * math.log2(160.0)) / 2
+    sign = torch.randint(0, 2, shape, generator=g) * 2.0 - 1.0
+    return (size * sign).to(device)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("T,E,H", [(1, 40, 70), (3, 7, 33), (70, 2, 66),
+                                   (1500, 1, 24), (5000, 1, 6)])
+@pytest.mark.parametrize("started", [False, True])
+def test_scan_of_far_gates(device, T, E, H, started):
+    """z x, (1 - z) h and z (1 - z) keep their relative accuracy however far
+    the gate is from zero: scan_64's bounds do not know its size."""
+    g = gen(T + H)
+    gate = far_gates(g, (T, E, H), device)
+    x, dhs = (randn(g, T, E, H, device=device) for _ in range(2))
+    h0, dhl = (randn(g, E, H, device=device) for _ in range(2))
+    done = (torch.rand(T, E, generator=g) < 0.1).to(device)
+    for d in (None, done):
+        args = (gate, x, h0 if started else None, d, dhs, dhl)
+        got, want = run_scan(*args), scan_64(*args)
+        for name in got:
+            close(got[name], *want[name], f"{name} {T}x{E}x{H}")
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("side", [-1.0, 1.0])
+def test_one_gate_at_a_time(device, side):
+    """Of a state and an input, each alone, what a far gate lets through: the
+    product of two values, each off by 8 u at most (as in scan_64), and one
+    rounding."""
+    gate = side * torch.linspace(0.5, 80.0, 4096).view(1, 1, -1).to(device)
+    one = torch.ones_like(gate)
+    hs, _ = gated_scan(gate, one)
+    z = torch.sigmoid(gate.double().cpu())
+    close(hs, z, 9 * U * z, "z")
+    kept, _ = gated_scan(gate, torch.zeros_like(gate), one[0])
+    a = torch.sigmoid(-gate.double().cpu())
+    close(kept, a, 9 * U * a, "1 - z")
+    h = torch.zeros_like(one[0])
+    close(gated_scan_step(gate[0], one[0], h), z[0], 9 * U * z[0], "step")
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_gates_at_the_ends(device):
+    """Infinite gates, gates whose e^-|gate| is 0, and NaN."""
+    v = torch.randn(1, 2, 6).to(device)
+    h = torch.randn(2, 6).to(device)
+    for far in (89.0, 104.0, 127.9, 128.0, 129.0, 1e4, 3e38, math.inf):
+        gate = torch.full_like(v, far)
+        # what is let through of the other side is below 2^-128 of it
+        assert torch.equal(gated_scan(gate, v, h)[0], v), far
+        assert torch.equal(gated_scan(-gate, v, h)[0], h[None]), far
+    bad = torch.full_like(v, math.nan)
+    assert gated_scan(bad, v, h)[0].isnan().all()
+    assert gated_scan(bad, v, h)[1].isnan().all()
