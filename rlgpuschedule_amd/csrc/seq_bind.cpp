@@ -484,8 +484,11 @@ Tensor scan_step(const Tensor& gate_, const Tensor& x_, Tensor h,
   const int type = check_scan(gate_, x_, h, done_, 2, "h");
   VALUE_CHECK(h.is_contiguous() && !h.is_neg(),
               "h is updated in place: it must be contiguous");
-  VALUE_CHECK(!h.requires_grad() || !at::GradMode::is_enabled(),
-              "h is updated in place and must not require a gradient");
+  no_tangent("gated_scan_step", {&gate_, &x_, &h});
+  VALUE_CHECK(!at::GradMode::is_enabled() ||
+                  !(wants_grad(gate_) || wants_grad(x_) || wants_grad(h)),
+              "gated_scan_step has no derivative: gate, x and h must not "
+              "require a gradient (call it under torch.no_grad())");
   for (const Tensor* t : {&gate_, &x_, given(done_)})
     VALUE_CHECK(!t || !h.is_alias_of(*t) ||
                     at::get_overlap_status(h, *t) == at::MemOverlapStatus::No,

@@ -54,14 +54,20 @@ def gated_scan_step(gate: torch.Tensor, x: torch.Tensor, h: torch.Tensor,
     """One acting step: gate, x [E, H]; h [E, H] f32 contiguous, UPDATED IN
     PLACE and sharing no memory with the others; done_prev [E] u8/bool marks
     environments whose state restarts from zero before this step. Returns the
-    output [E, H] in x's type. Not differentiable."""
+    output [E, H] in x's type. Not differentiable: under grad mode gate, x and
+    h that require a gradient are refused, and tangents always."""
     if x.is_cuda:
         return ext().gated_scan_step(gate, x, h, done_prev)
     if not h.is_contiguous():
         raise ValueError("h is updated in place: it must be contiguous")
-    if h.requires_grad and torch.is_grad_enabled():
-        raise ValueError("h is updated in place and must not require a "
-                         "gradient")
+    for t in (gate, x, h):
+        if torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError("gated_scan_step has no forward-mode "
+                               "derivative")
+        if t.requires_grad and torch.is_grad_enabled():
+            raise ValueError("gated_scan_step has no derivative: gate, x and "
+                             "h must not require a gradient (call it under "
+                             "torch.no_grad())")
     with torch.no_grad():
         c = h if done_prev is None else h.masked_fill(
             done_prev.unsqueeze(-1) != 0, 0.0)

@@ -128,3 +128,34 @@ def test_gates_at_the_ends(device):
     bad = torch.full_like(v, math.nan)
     assert gated_scan(bad, v, h)[0].isnan().all()
     assert gated_scan(bad, v, h)[1].isnan().all()
+
+
+# ------------------------------------------------- what a step would lose
+@pytest.mark.parametrize("device", DEVICES)
+def test_step_refuses_gradients_and_tangents(device):
+    """A step has no derivative: gate, x and h that want one are refused where
+    it would be dropped, and taken where none is recorded."""
+    v = torch.randn(3, 8).to(device)
+    h = torch.zeros(3, 8, device=device)
+    for i in range(3):
+        args = [v.clone(), v.clone(), h.clone()]
+        args[i].requires_grad_(True)
+        with pytest.raises(ValueError, match="gradient"):
+            gated_scan_step(*args)
+        with pytest.raises(ValueError, match="gradient"):
+            gated_scan_step((args[0] * 1), (args[1] * 1), args[2] * 1)
+        with torch.no_grad():
+            gated_scan_step(*args)
+        with torch.inference_mode():
+            gated_scan_step(args[0], args[1], h.clone())
+    with torch.autograd.forward_ad.dual_level():
+        for i in range(3):
+            args = [v.clone(), v.clone(), h.clone()]
+            args[i] = torch.autograd.forward_ad.make_dual(
+                args[i], torch.ones_like(v))
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                gated_scan_step(*args)
+            with torch.no_grad(), pytest.raises(RuntimeError,
+                                                match="forward-mode"):
+                gated_scan_step(*args)
+    assert torch.equal(h, torch.zeros_like(h))
