@@ -30,9 +30,9 @@ def compute_gae(buf: RolloutBuffer, gamma: float, lam: float):
 def replay_sequence(policy, obs, mask, actions, h0, done):
     """Log probabilities, entropies and values [T, E] of a recurrent policy
     along stored sequences, from h0 and with its state reset at the stored
-    done flags. Policies with forward_sequence replay all of it at once,
-    others step by step."""
-    if hasattr(policy, "forward_sequence"):
+    done flags. Sequence policies (is_sequence_policy) replay all of it at
+    once, others step by step."""
+    if getattr(policy, "is_sequence_policy", False):
         logits, value, _ = policy.forward_sequence(obs, h0, done)
         r = action_logprobs(logits, actions, mask)
         return r.logp, r.entropy, value

@@ -64,7 +64,7 @@ class Collector:
         self.obs = env.reset().to(torch.float32)
         self.mask = env.action_masks()
         self.hx = policy.initial_state(env.num_envs, self.device)
-        # policies with step() keep their state in place, and reset it
+        # sequence policies keep their state in place, and reset it
         # themselves where the step before ended an episode
         self.done_prev = None
         hidden = policy.hidden if policy.is_recurrent else 0
@@ -74,7 +74,7 @@ class Collector:
     @torch.no_grad()
     def collect(self) -> RolloutBuffer:
         buf = self.buf
-        in_place = hasattr(self.policy, "step")
+        in_place = getattr(self.policy, "is_sequence_policy", False)
         if buf.h0 is not None:
             buf.h0.copy_(self.hx)
             if in_place and self.done_prev is not None:

@@ -94,6 +94,8 @@ class LinearRecurrentPolicy(nn.Module):
     kernels on the GPU (ops/norm.py, ops/scan.py)."""
 
     is_recurrent = True
+    # collectors act by step() and learners replay by forward_sequence()
+    is_sequence_policy = True
 
     def __init__(self, obs_dim: int, num_actions: int, hidden: int = 256):
         super().__init__()
