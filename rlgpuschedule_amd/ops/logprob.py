@@ -4,9 +4,9 @@ and backward, for any number of actions.
 
 An action that the mask leaves out is the same as one of logit -inf:
 probability 0, no gradient, never an alternative, whatever its logit holds.
-On CPU tensors `action_logprobs` runs the torch reference (ops/seq_ref.py).
-Launches go to the current stream of the logits' device and are
-hipGraph-capturable."""
+On CPU tensors `action_logprobs` runs the torch reference (ops/seq_ref.py)
+after the same checks. Launches go to the current stream of the logits' device
+and are hipGraph-capturable."""
 from __future__ import annotations
 
 from typing import NamedTuple
@@ -14,9 +14,8 @@ from typing import NamedTuple
 import torch
 
 from ._seq import ext
+from ._seq_checks import MAX_TOP_K, check_logp  # noqa: F401
 from .seq_ref import action_logprobs_reference
-
-MAX_TOP_K = 64
 
 
 class LogProbs(NamedTuple):
@@ -67,7 +66,5 @@ def action_logprobs(logits: torch.Tensor, actions: torch.Tensor,
       top_k (at most 64) have a logit above -inf, the rest are (-inf, -1)."""
     if logits.is_cuda:
         return LogProbs(*ext().action_logprobs(logits, actions, mask, top_k))
-    if not 0 <= top_k <= min(MAX_TOP_K, logits.shape[-1]):
-        raise ValueError(f"top_k must be 0 to {MAX_TOP_K} and at most the "
-                         f"number of actions, got {top_k}")
+    check_logp(logits, actions, mask, top_k)
     return LogProbs(*action_logprobs_reference(logits, actions, mask, top_k))

@@ -3,13 +3,14 @@
 `layer_norm` is the differentiable call; `layer_norm_fwd` and
 `layer_norm_bwd` are the explicit pair for learners that capture their
 update. On CPU tensors `layer_norm` runs the torch reference
-(ops/seq_ref.py). Launches go to the current stream of x's device and are
+(ops/seq_ref.py) after the same checks. Launches go to the current stream of x's device and are
 hipGraph-capturable."""
 from __future__ import annotations
 
 import torch
 
 from ._seq import ext
+from ._seq_checks import check_norm
 from .seq_ref import layer_norm_reference
 
 
@@ -41,4 +42,5 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None,
     held in 32 bits; y has x's type."""
     if x.is_cuda:
         return ext().layer_norm(x, weight, bias, eps)
+    check_norm(x, weight, bias)
     return layer_norm_reference(x, weight, bias, eps)

@@ -8,13 +8,14 @@ Time-major [T, E, H] with done [T, E] u8 marking the steps that ended an
 episode, as the rollout buffers have them: h_last is the carry of the next
 rollout, and sequences of different lengths can lie one behind the other.
 The state is float32 throughout. On CPU tensors gated_scan and
-gated_scan_step run the torch reference (ops/seq_ref.py). Launches go to the
-current stream of x's device and are hipGraph-capturable."""
+gated_scan_step run the torch reference (ops/seq_ref.py) after the same checks.
+Launches go to the current stream of x's device and are hipGraph-capturable."""
 from __future__ import annotations
 
 import torch
 
 from ._seq import ext
+from ._seq_checks import check_scan, check_step
 from .seq_ref import gated_scan_reference
 
 
@@ -46,6 +47,7 @@ def gated_scan(gate: torch.Tensor, x: torch.Tensor,
     and h0; arguments as gated_scan_fwd's."""
     if x.is_cuda:
         return ext().gated_scan(gate, x, h0, done)
+    check_scan(gate, x, h0, done, 3, "h0")
     return gated_scan_reference(gate, x, h0, done)
 
 
@@ -58,16 +60,7 @@ def gated_scan_step(gate: torch.Tensor, x: torch.Tensor, h: torch.Tensor,
     h that require a gradient are refused, and tangents always."""
     if x.is_cuda:
         return ext().gated_scan_step(gate, x, h, done_prev)
-    if not h.is_contiguous():
-        raise ValueError("h is updated in place: it must be contiguous")
-    for t in (gate, x, h):
-        if torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
-            raise RuntimeError("gated_scan_step has no forward-mode "
-                               "derivative")
-        if t.requires_grad and torch.is_grad_enabled():
-            raise ValueError("gated_scan_step has no derivative: gate, x and "
-                             "h must not require a gradient (call it under "
-                             "torch.no_grad())")
+    check_step(gate, x, h, done_prev)
     with torch.no_grad():
         c = h if done_prev is None else h.masked_fill(
             done_prev.unsqueeze(-1) != 0, 0.0)

@@ -5,7 +5,8 @@ import math
 import pytest
 import torch
 
-from rlgpuschedule_amd import gated_scan, gated_scan_step, layer_norm
+from rlgpuschedule_amd import (action_logprobs, gated_scan, gated_scan_step,
+                               layer_norm)
 from rlgpuschedule_amd.ops.norm import layer_norm_bwd, layer_norm_fwd
 
 from test_seq_ops import (DEVICES, U, close, gen, randn, run_scan,
@@ -159,3 +160,135 @@ def test_step_refuses_gradients_and_tangents(device):
                                                 match="forward-mode"):
                 gated_scan_step(*args)
     assert torch.equal(h, torch.zeros_like(h))
+
+
+# ----------------------------------------------- refusals of the public calls
+def norm_refusals(t):
+    x = t(4, 8)
+    return [
+        (ValueError, lambda: layer_norm(t())),
+        (ValueError, lambda: layer_norm(t(4, 0))),
+        (TypeError, lambda: layer_norm(x.long())),
+        (TypeError, lambda: layer_norm(x.bool())),
+        (ValueError, lambda: layer_norm(x, t(1))),
+        (ValueError, lambda: layer_norm(x, t(7))),
+        (ValueError, lambda: layer_norm(x, t(1, 8))),
+        (ValueError, lambda: layer_norm(x, None, t(4, 8))),
+        (TypeError, lambda: layer_norm(x, t(8).half())),
+        (TypeError, lambda: layer_norm(x.bfloat16(), t(8).half())),
+        (TypeError, lambda: layer_norm(x, t(8).double())),
+        (TypeError, lambda: layer_norm(x.half(), t(8).half(), t(8))),
+        (ValueError, lambda: layer_norm(x, t(8).to("meta"))),
+        (ValueError, lambda: layer_norm(x, None, t(8).to("meta"))),
+    ]
+
+
+def scan_refusals(t):
+    x, h, d = t(4, 2, 6), t(2, 6), t(4, 2).bool()
+    many = t(1).expand(1, 1 << 16, 1 << 15)
+    base = t(2, 20)
+    return [
+        (ValueError, lambda: gated_scan(x[0], x[0])),
+        (ValueError, lambda: gated_scan(t(4, 2, 5), x)),
+        (ValueError, lambda: gated_scan(t(1, 2, 6), x)),
+        (ValueError, lambda: gated_scan(x.half(), x)),
+        (TypeError, lambda: gated_scan(x.long(), x.long())),
+        (ValueError, lambda: gated_scan(many, many)),
+        (ValueError, lambda: gated_scan(x, x, h.half())),
+        (ValueError, lambda: gated_scan(x, x, h.double())),
+        (ValueError, lambda: gated_scan(x.half(), x.half(), h.half())),
+        (ValueError, lambda: gated_scan(x, x, t(6))),
+        (ValueError, lambda: gated_scan(x, x, t(2, 5))),
+        (ValueError, lambda: gated_scan(x, x, h.to("meta"))),
+        (ValueError, lambda: gated_scan(x.to("meta"), x)),
+        (ValueError, lambda: gated_scan(x, x, h, t(4, 2))),
+        (ValueError, lambda: gated_scan(x, x, h, t(4, 1).bool())),
+        (ValueError, lambda: gated_scan(x, x, h, d.t())),
+        (ValueError, lambda: gated_scan(x, x, h, d.to("meta"))),
+        (ValueError, lambda: gated_scan_step(x, x, h)),
+        (ValueError, lambda: gated_scan_step(x[0], x[0], h.half())),
+        (ValueError, lambda: gated_scan_step(x[0].half(), x[0].half(),
+                                             h.half())),
+        (ValueError, lambda: gated_scan_step(x[0], x[0], t(6))),
+        (ValueError, lambda: gated_scan_step(x[0], x[0], t(2, 12)[:, ::2])),
+        (ValueError, lambda: gated_scan_step(x[0], x[0], t(6, 2).t())),
+        (ValueError, lambda: gated_scan_step(x[0], x[0], h, d)),
+        (ValueError, lambda: gated_scan_step(x[0], x[0], h, d[0].float())),
+        # h in memory that the others are read from
+        (ValueError, lambda: gated_scan_step(h, x[0], h)),
+        (ValueError, lambda: gated_scan_step(x[0], h, h)),
+        (ValueError, lambda: gated_scan_step(
+            x[0], x[0], h, h.view(torch.uint8).view(-1)[:2])),
+        (ValueError, lambda: gated_scan_step(
+            base.view(-1)[4:16].view(2, 6), x[0],
+            base.view(-1)[:12].view(2, 6))),
+        (ValueError, lambda: gated_scan_step(
+            base[:, 14:], x[0], base.view(-1)[:12].view(2, 6))),
+    ]
+
+
+def logp_refusals(t):
+    x, a = t(4, 8), t(4).long()
+    return [
+        (ValueError, lambda: action_logprobs(t(), a)),
+        (ValueError, lambda: action_logprobs(t(4, 0), a)),
+        (ValueError, lambda: action_logprobs(
+            t(1).expand(4, (1 << 30) + 1), a)),
+        (TypeError, lambda: action_logprobs(x.long(), a)),
+        (ValueError, lambda: action_logprobs(x, a[:3])),
+        (ValueError, lambda: action_logprobs(x, a[:1])),
+        (ValueError, lambda: action_logprobs(x, a.int())),
+        (ValueError, lambda: action_logprobs(x, a.view(4, 1))),
+        (ValueError, lambda: action_logprobs(x, a, t(4, 7).bool())),
+        (ValueError, lambda: action_logprobs(x, a, t(8).bool())),
+        (ValueError, lambda: action_logprobs(x, a, t(1, 8).bool())),
+        (ValueError, lambda: action_logprobs(x, a, t(4, 8))),
+        (ValueError, lambda: action_logprobs(x, a, t(4, 8).bool().to("meta"))),
+        (ValueError, lambda: action_logprobs(x, a.to("meta"))),
+        (ValueError, lambda: action_logprobs(x, a, top_k=9)),
+        (ValueError, lambda: action_logprobs(x, a, top_k=-1)),
+        (ValueError, lambda: action_logprobs(t(4, 100), a, top_k=65)),
+    ]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("cases", [norm_refusals, scan_refusals,
+                                   logp_refusals])
+@pytest.mark.parametrize("grad", [False, True])
+def test_public_calls_refuse_alike(device, cases, grad):
+    """What one device refuses the other refuses, with the same kind of
+    error, whether or not a gradient is asked for."""
+    def t(*size):
+        return torch.zeros(size, device=device)
+
+    with torch.set_grad_enabled(grad):
+        for i, (error, call) in enumerate(cases(t)):
+            with pytest.raises(error):
+                call()
+                pytest.fail(f"case {i} was taken")
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_step_takes_a_state_beside_its_inputs(device):
+    """Views of one allocation that lie apart are taken."""
+    base = torch.randn(36).to(device)
+    gate, x, h = (base[i:i + 12].view(2, 6) for i in (0, 12, 24))
+    want = h.clone()
+    out = gated_scan_step(gate.clone(), x.clone(), want)
+    assert torch.equal(gated_scan_step(gate, x, h), out)
+    assert torch.equal(h, want)
+
+
+def test_float64_on_the_cpu():
+    """float64 inputs work there in 64 bits, states included."""
+    g = gen(9)
+    gate, x = (randn(g, 5, 2, 6).double() for _ in range(2))
+    h = randn(g, 2, 6).double()
+    hs, last = gated_scan(gate, x, h)
+    assert hs.dtype == last.dtype == torch.float64
+    steps = torch.stack([gated_scan_step(gate[t], x[t], h) for t in range(5)])
+    assert torch.equal(steps, hs) and torch.equal(h, last)
+    w = randn(g, 6).double()
+    assert layer_norm(x, w, w).dtype == torch.float64
+    act = torch.zeros(5, 2, dtype=torch.int64)
+    assert action_logprobs(x, act).logp.dtype == torch.float64
