@@ -105,9 +105,9 @@ struct ScanBwd {
 
 // e^-|g|, to its own last bits: of m = |g|, e^-m = 2^p (1 + t), p the rounded
 // product -m / ln 2 and t = -m - p ln 2 what its rounding left out. Without t
-// it is off by up to m half steps, and with it the smaller of z and 1 - z. Three
-// instructions, of which a small call sees most: 512x32x256 bf16 takes 14.4 us
-// forward instead of 13.9, 65x64x256 6.8 instead of 6.6.
+// it is off by up to m half steps, and with it the smaller of z and 1 - z.
+// That is three instructions, of which a small call sees most: 512x32x256 bf16
+// takes 14.4 us forward instead of 13.9, 65x64x256 6.8 instead of 6.6.
 __device__ __forceinline__ float decay(float g) {
   constexpr double kLn2 = 0.69314718055994530942;
   constexpr float kHigh = (float)kLn2, kLow = (float)(kLn2 - (double)kHigh);
@@ -188,30 +188,30 @@ __device__ __forceinline__ void read_steps(Vec<T, V> (&to)[N], const T* from,
   }
 }
 
-// Which of N steps end an episode: their flags as they are read, and before the
-// rest, so that nothing waits for them alone: 256x1024x256 bf16 takes 83 us
+// Which of kKeep steps end an episode: their flags as they are read, and before
+// the rest, so that nothing waits for them alone: 256x1024x256 bf16 takes 83 us
 // forward so, and 95 where they are made bits of one word behind it.
-template <int N>
 struct Ends {
-  uint8_t flags[N];
+  uint8_t flags[kKeep];
 
   template <bool FULL>
   __device__ __forceinline__ void read(const uint8_t* done, int64_t E,
                                        const Lane& l, int64_t t, int64_t end) {
     const uint8_t* at = done + t * E + l.e0 + l.e;
 #pragma unroll
-    for (int k = 0; k < N; ++k) flags[k] = FULL || t + k < end ? at[k * E] : 0;
+    for (int k = 0; k < kKeep; ++k)
+      flags[k] = FULL || t + k < end ? at[k * E] : 0;
   }
   __device__ __forceinline__ bool operator[](int k) const {
     return flags[k] != 0;
   }
 };
 
-// L steps of a lane's columns, and which of them end an episode.
-template <typename T, int V, int L>
+// kKeep steps of a lane's columns, and which of them end an episode.
+template <typename T, int V>
 struct Steps {
-  Vec<T, V> gate[L], x[L];
-  Ends<L> ends;
+  Vec<T, V> gate[kKeep], x[kKeep];
+  Ends ends;
 
   template <bool FULL, bool DONE>
   __device__ __forceinline__ void read(const ScanFwd& p, const Lane& l,
@@ -222,16 +222,16 @@ struct Steps {
   }
 };
 
-template <bool FULL, bool DONE, typename T, int V, int L>
+template <bool FULL, bool DONE, typename T, int V>
 __device__ __forceinline__ void walk(const ScanFwd& p, const Lane& l,
-                                     const Steps<T, V, L>& s, int64_t t,
+                                     const Steps<T, V>& s, int64_t t,
                                      int64_t end, float (&c)[V]) {
   const int64_t EH = p.c.E * p.c.H;
-  if (p.states && t % kKeep == 0)
+  if (p.states)
     store<float, V>(here(p.states + t / kKeep * EH, l, p.c.H), c);
   T* out = here((T*)p.hs + t * EH, l, p.c.H);
 #pragma unroll
-  for (int k = 0; k < L; ++k) {
+  for (int k = 0; k < kKeep; ++k) {
     if (!FULL && t + k >= end) continue;
     float h[V];
 #pragma unroll
@@ -245,11 +245,10 @@ __device__ __forceinline__ void walk(const ScanFwd& p, const Lane& l,
   }
 }
 
-// kKeep is a multiple of L and a chunk one of kKeep, so states lie at the
-// first of L steps.
-template <typename T, int V, int L, bool DONE>
+// A chunk is a multiple of kKeep, so states are kept where steps are read.
+template <typename T, int V, bool DONE>
 __global__ __launch_bounds__(256) void scan_fwd_kernel(ScanFwd p) {
-  static_assert(kKeep % L == 0, "states are kept between steps read at once");
+  constexpr int L = kKeep;
   Lane l;
   if (!lane_of<V>(p.c, l)) return;
   const int64_t EH = p.c.E * p.c.H;
@@ -264,7 +263,7 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(ScanFwd p) {
   if (p.ways) follow<V>(p.ways, p.c, l, 0, blockIdx.y, false, c);
   if (t + L <= end) {
     // the next steps are read while these are walked
-    Steps<T, V, L> s, n;
+    Steps<T, V> s, n;
     s.template read<true, DONE>(p, l, t, end);
     for (; t + 2 * L <= end; t += L) {
       n.template read<true, DONE>(p, l, t + L, end);
@@ -275,20 +274,20 @@ __global__ __launch_bounds__(256) void scan_fwd_kernel(ScanFwd p) {
     t += L;
   }
   if (t < end) {
-    Steps<T, V, L> s;
+    Steps<T, V> s;
     s.template read<false, DONE>(p, l, t, end);
     walk<false, DONE>(p, l, s, t, end, c);
   }
   if (end == p.T) store<float, V>(here(p.h_last, l, p.c.H), c);
 }
 
-template <bool FULL, bool DONE, typename T, int V, int L>
+template <bool FULL, bool DONE, typename T, int V>
 __device__ __forceinline__ void way(const ScanFwd& p, const Lane& l, int64_t t,
                                     int64_t end, Way (&w)[V]) {
-  Steps<T, V, L> s;
+  Steps<T, V> s;
   s.template read<FULL, DONE>(p, l, t, end);
 #pragma unroll
-  for (int k = 0; k < L; ++k) {
+  for (int k = 0; k < kKeep; ++k) {
     if (!FULL && t + k >= end) continue;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
@@ -326,8 +325,8 @@ __global__ __launch_bounds__(256) void scan_fwd_way_kernel(ScanFwd p,
   int64_t t = from_last() * p.chunk;
   const int64_t end = t + p.chunk < p.T ? t + p.chunk : p.T;
   Way w[V];
-  for (; t + L <= end; t += L) way<true, DONE, T, V, L>(p, l, t, end, w);
-  if (t < end) way<false, DONE, T, V, L>(p, l, t, end, w);
+  for (; t + L <= end; t += L) way<true, DONE, T, V>(p, l, t, end, w);
+  if (t < end) way<false, DONE, T, V>(p, l, t, end, w);
   keep_way<V>(p.c, l, w, ways);
 }
 
@@ -414,7 +413,7 @@ __device__ __forceinline__ Vec<T, V> masked(Vec<T, V> x, uint32_t bits) {
 template <typename T, int V>
 struct Back {
   Vec<T, V> gate[kKeep], dhs[kKeep];
-  Ends<kKeep> ends;
+  Ends ends;
 
   template <bool FULL, bool DONE>
   __device__ __forceinline__ void read(const ScanBwd& p, const Lane& l,
@@ -701,7 +700,7 @@ hipError_t fwd_with(const ScanFwd& p, const Plan& q, float* ways,
       e = join(ways, p.h0, p.carry, q, EH, false, s);
     if (e != hipSuccess) return e;
   }
-  return launch(scan_fwd_kernel<T, V, kKeep, DONE>, grid, dim3(256), 0, s, p);
+  return launch(scan_fwd_kernel<T, V, DONE>, grid, dim3(256), 0, s, p);
 }
 
 template <typename T>

@@ -958,8 +958,8 @@ Group group_of(int64_t A, int V) {
 // 51 us, 8192 x 2048 fp32 with 20 25 and 33 (16 bits to 8: 8192 x 4096 with 20
 // 38 and 37).
 constexpr int64_t kGroupVecs = 4 * kWave;
-constexpr int64_t group_vecs(int k, int V) {
-  return (V == 4 ? k ? 8 : 6 : k ? 6 : 4) * kWave;
+constexpr int64_t group_vecs(bool top, int V) {
+  return (V == 4 ? top ? 8 : 6 : top ? 6 : 4) * kWave;
 }
 
 template <typename T, bool BWD, int G, int N, typename P>
@@ -967,12 +967,17 @@ hipError_t group_with(const P& p, hipStream_t s) {
   constexpr int B = 256;
   const int64_t want = (p.rows + B / G - 1) / (B / G);
   const dim3 grid(want < kGrid ? want : kGrid);
+  // only what rows of so many vectors come to is built
   if constexpr (BWD) {
+    static_assert(G * N <= kGroupVecs);
     return launch(logp_group_bwd_kernel<T, G, N>, grid, dim3(B), 0, s, p);
   } else {
+    static_assert(G * N <= group_vecs(true, kVec<T>));
     if (p.k)
       return launch(logp_group_kernel<T, G, N, true>, grid, dim3(B), 0, s, p);
-    return launch(logp_group_kernel<T, G, N, false>, grid, dim3(B), 0, s, p);
+    if constexpr (G * N <= group_vecs(false, kVec<T>))
+      return launch(logp_group_kernel<T, G, N, false>, grid, dim3(B), 0, s, p);
+    return hipErrorInvalidValue;
   }
 }
 
@@ -981,7 +986,8 @@ hipError_t group(const P& p, hipStream_t s) {
   const Group g = group_of(p.A, kVec<T>);
   if constexpr (!BWD) {
     if (g.N == 6) return group_with<T, false, 64, 6>(p, s);
-    if (g.N == 8) return group_with<T, false, 64, 8>(p, s);
+    if constexpr (64 * 8 <= group_vecs(true, kVec<T>))
+      if (g.N == 8) return group_with<T, false, 64, 8>(p, s);
   }
   switch (g.G * 8 + g.N) {
     case 1 * 8 + 1: return group_with<T, BWD, 1, 1>(p, s);
@@ -1013,7 +1019,7 @@ hipError_t group(const P& p, hipStream_t s) {
 constexpr int64_t kWhole = 2048;
 constexpr int64_t kBlocks = 512;
 
-int parts_of(int64_t rows, int64_t A, int k, int V) {
+int parts_of(int64_t rows, int64_t A, int V) {
   const int64_t n = (A + V - 1) / V;
   if (n <= kWhole || rows <= 0) return 1;
   int64_t p = (kBlocks + rows - 1) / rows;
@@ -1027,7 +1033,7 @@ hipError_t fwd(const LogpFwd& p, void* scratch, int type, hipStream_t s) {
   if (p.rows == 0) return hipSuccess;
   const int64_t n = (p.A + kVec<T> - 1) / kVec<T>;
   if (n <= group_vecs(p.k, kVec<T>)) return group<T, false>(p, s);
-  const int P = parts_of(p.rows, p.A, p.k, kVec<T>);
+  const int P = parts_of(p.rows, p.A, kVec<T>);
   const int64_t blocks = p.rows * P;
   const Parts parts = {(float*)((uint64_t*)scratch + blocks * p.k),
                        (uint64_t*)scratch, P};
@@ -1066,7 +1072,7 @@ hipError_t bwd(const LogpBwd& p, hipStream_t s) {
 // Bytes of scratch that the forward call needs.
 extern "C" int64_t rlsched_logp_scratch(int64_t rows, int64_t A, int k,
                                         int type) {
-  const int P = parts_of(rows, A, k, type == F32 ? 4 : 8);
+  const int P = parts_of(rows, A, type == F32 ? 4 : 8);
   return P == 1 ? 0 : rows * P * (8 * (int64_t)k + 12);
 }
 
