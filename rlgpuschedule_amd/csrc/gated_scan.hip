@@ -556,9 +556,9 @@ __global__ __launch_bounds__(256) void scan_bwd_kernel(ScanBwd p) {
   } else {
     for (; t >= t0; t -= kKeep) {
       now.template read<true, DONE>(p, l, t, end);
-      // No read is put off until a register is free: without ends 64x2048x256
-      // bf16 takes 74 us so and 78 otherwise (with ends 64x1024x256 40 and 38).
-      __builtin_amdgcn_sched_barrier(0);
+      // No read is put off until a register is free: 64x2048x256 bf16 takes 74
+      // us so and 78 otherwise. With ends, or in 32 bits, none is.
+      if constexpr (sizeof(T) == 2 && !DONE) __builtin_amdgcn_sched_barrier(0);
       walk_back<true, DONE>(p, l, now, t, end, carry);
     }
   }
