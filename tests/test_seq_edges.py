@@ -292,3 +292,30 @@ def test_float64_on_the_cpu():
     assert layer_norm(x, w, w).dtype == torch.float64
     act = torch.zeros(5, 2, dtype=torch.int64)
     assert action_logprobs(x, act).logp.dtype == torch.float64
+
+
+# ---------------------------------------------------------- the first call
+def test_threads_that_load_the_bindings_at_once(monkeypatch):
+    """The first calls of several threads build and load the bindings once."""
+    import threading
+    import time
+
+    from rlgpuschedule_amd.ops import _seq
+    built, real = [], _seq.build_lib
+
+    def slow(name):
+        built.append(name)
+        time.sleep(0.05)
+        return real(name)
+
+    monkeypatch.setattr(_seq, "build_lib", slow)
+    monkeypatch.setattr(_seq, "_ext", None)
+    got = []
+    threads = [threading.Thread(target=lambda: got.append(_seq.ext()))
+               for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(got) == 4 and all(m is got[0] for m in got)
+    assert sorted(built) == sorted(set(built))
