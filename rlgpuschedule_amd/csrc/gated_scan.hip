@@ -667,6 +667,7 @@ Plan plan(int64_t T, int64_t E, int64_t H, int bytes, bool back) {
 // too much (2063x3x64 fp32's 129: 20 us instead of 12.5): scratch then holds
 // the chunks' starts as well.
 constexpr int64_t kFollow = 64;
+static_assert(kFollow >= 1, "a call that is not cut has no scratch");
 
 template <typename P>
 void give_ways(P& p, const Plan& q, float* scratch) {
