@@ -17,12 +17,16 @@
 // state, c_end = A c_start + B, those are joined from chunk to chunk, and a
 // last kernel walks every chunk from its own start.
 //
-// Bound by memory where it is walked: 64 x 2048 x 256 bf16 takes 46 us forward
-// (217 MB with the kept states, 4.7 TB/s) and 70 us backward (352 MB, 5.0), a
-// large copy's rate being 4.9. In chunks gate and x are read twice: 32768 x 2
-// x 1000 takes 70 us for the effects (262 MB; reading alone runs at 4.0 TB/s),
-// 8 to join 512 chunks and 64 to walk. Small calls are bound by the latency
-// of kKeep steps after another: 65 x 64 x 256 bf16 takes 7.5 and 11 us.
+// Bound by memory where it is walked: 64 x 2048 x 256 bf16 with ends takes 44
+// us forward (218 MB with the kept states, 5.0 TB/s) and 66 us backward (352
+// MB, 5.3; part of both lies in the 256 MB cache), a large copy's rate being
+// 4.9. In chunks gate and x are read twice: 32768 x 2 x 1000 takes 68 us for
+// the effects (262 MB), 9 to join 512 chunks and 68 to walk. Small calls are
+// bound by the latency of kKeep steps after another: 65 x 64 x 256 bf16 with
+// ends takes 7.5 and 11 us.
+//
+// In chunks a state that has become infinite may go on as NaN: the product of
+// a chunk's a may be 0 where none of them is, and 0 times an infinity is NaN.
 #include "seq_api.h"
 #include "seq_common.h"
 
@@ -30,8 +34,8 @@ namespace {
 using namespace seq;
 
 // Steps from one kept state to the next: what the backward pass holds at once.
-// 16 of them took twice the registers for half as wide loads: 128 us instead
-// of 112 for a training pass of 64 x 2048 x 256 bf16.
+// 16 of them took twice the registers for half as wide loads, and a training
+// pass of 64 x 2048 x 256 bf16 a seventh longer.
 constexpr int kKeep = 8;
 
 // A sequence's columns as lanes: n lanes an environment, the last of which
@@ -107,7 +111,8 @@ struct ScanBwd {
 // product -m / ln 2 and t = -m - p ln 2 what its rounding left out. Without t
 // it is off by up to m half steps, and with it the smaller of z and 1 - z.
 // That is three instructions, of which a small call sees most: 512x32x256 bf16
-// takes 14.4 us forward instead of 13.9, 65x64x256 6.8 instead of 6.6.
+// takes 14.4 us forward instead of 13.9, 65x64x256 6.8 instead of 6.6 (without
+// ends).
 __device__ __forceinline__ float decay(float g) {
   constexpr double kLn2 = 0.69314718055994530942;
   constexpr float kHigh = (float)kLn2, kLow = (float)(kLn2 - (double)kHigh);
@@ -622,16 +627,16 @@ constexpr int64_t kShort = 64;    // steps that one lane walks in any case
 
 // Lanes take 8 bytes of columns, as few load instructions as the memory's
 // rate allows, or fewer where that leaves too few waves: 64x256x256 bf16 runs
-// in 9.3 us forward and 18.8 us backward with 2 bytes, in 17.3 and 30.4 us
-// with 8; 64x1024x256 in 24 and 39 us with 8.
+// in 10.2 us forward and 19 us backward with 2 bytes, in 19 and 26 us with 8;
+// 64x1024x256 in 24 and 38 us with 8. (Here and below with ends.)
 //
 // Time is cut where a lane would walk more than kShort steps among few waves:
-// 512x32x256 bf16 runs in 14 and 22 us in chunks, in 47 and 106 us walked;
-// 65x64x256 in 7.5 and 11 us instead of 9 and 16; 32x64x64 fp32 would take 6.6
-// and 9.4 instead of 5.0 and 8.6. With 1024 waves it is
-// walked (256x1024x256 bf16: 92 and 164 us, in chunks 162 and 241, which read
-// more), but backward not by lanes of 2 bytes (512x256x256 bf16: 64 us walked
-// forward, 75 in chunks; 134 us walked backward, 109 in chunks).
+// 512x32x256 bf16 runs in 16 and 22 us in chunks, in 48 and 113 us walked;
+// 65x64x256 in 7.5 and 11 us instead of 9 and 19; 32x64x64 fp32 would take 6.7
+// and 8.9 instead of 5.0 and 8.7. With 1024 waves it is walked (256x1024x256
+// bf16: 83 and 135 us, in chunks 142 and 191, which read more), but backward
+// not by lanes of 2 bytes (512x256x256 bf16: 64 us walked forward, 80 in
+// chunks; 141 us walked backward, 106 in chunks).
 Plan plan(int64_t T, int64_t E, int64_t H, int bytes, bool back) {
   Plan p;
   int64_t waves = 0;
@@ -662,9 +667,9 @@ Plan plan(int64_t T, int64_t E, int64_t H, int bytes, bool back) {
 }
 
 // A chunk follows the ways of up to kFollow others itself, without a kernel
-// between: 509x37x263 fp16's 22 chunks are walked 4 us sooner each way,
-// 663x36x64 bf16's 42 0.3 and 0.9 us, and a launch is saved. More would read
-// too much (2063x3x64 fp32's 129: 20 us instead of 12.5): scratch then holds
+// between: 509x37x263 fp16's 22 chunks are walked 4.5 us sooner each way,
+// 663x36x64 bf16's 42 0.8 and 1.4 us, and a launch is saved. More would read
+// too much (2063x3x64 fp32's 129: 19 us instead of 12.3): scratch then holds
 // the chunks' starts as well.
 constexpr int64_t kFollow = 64;
 static_assert(kFollow >= 1, "a call that is not cut has no scratch");

@@ -8,11 +8,15 @@
 // Statistics and sums are held in 32 bits; y, dx, dw and db are rounded to
 // their types once.
 //
-// Bound by memory: x is read once by each pass and held in registers between
-// the sums and what needs them, dy likewise. On an MI355X, whose large copy
-// runs at 4.9 TB/s, 131072 x 256 bf16 takes 27 us forward (5.0 TB/s) and 37
-// us backward (5.5 TB/s, the last sum among it), 8192 x 4096 fp16 26 and 44
-// us; 256 x 256 fp32 takes 2.7 us, a launch's time.
+// Bound by memory: of rows of up to 2048 vectors of 16 bytes x is read once by
+// each pass and held in registers between the sums and what needs them, dy
+// likewise. On an MI355X, whose large copy runs at 4.9 TB/s, 131072 x 256 bf16
+// takes 30.5 us forward (4.4 TB/s) and 34 + 4 us backward (the last sum of dw
+// and db apart; 5.3 TB/s, partly from the cache), 8192 x 4096 fp16 34 and 40 +
+// 4 us; 256 x 256 fp32 takes 3.2 us, a launch's time. Longer rows are walked by
+// a block, an element a lane, x three times forward, x and dy three times
+// backward: 2048 x 8192 fp32 takes 26 and 38 us, 2048 x 8200 40 and 82, 1024 x
+// 16384 41 and 72.
 #include "seq_api.h"
 #include "seq_common.h"
 

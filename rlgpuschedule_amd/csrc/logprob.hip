@@ -10,11 +10,13 @@
 // m and log s are kept apart: where every logit is the type's lowest value,
 // their sum would lose log s.
 //
+// A probability below 2^-126 counts as 0.
+//
 // Bound by memory: one pass over the logits each way. On an MI355X 4096 x
-// 32768 bf16 takes 72 us forward (268 MB; reading alone runs at 4.0 TB/s
-// there) and 110 us backward (537 MB, 4.9 TB/s, a large copy's rate); 524288
-// x 17 fp32 with a mask 15 and 25 us. One row of 131072 with 20 alternatives
-// takes 7 us in 32 parts and 6 to join them, its latency.
+// 32768 bf16 takes 75 us forward (268 MB, 3.6 TB/s; a large sum of torch's
+// reads at 4.0 there) and 114 us backward (537 MB, 4.7 TB/s; a large copy's
+// rate is 4.9); 524288 x 17 fp32 with a mask 16 and 25 us. One row of 131072
+// with 20 alternatives takes 7 us in 32 parts and 5 to join them, its latency.
 #include "seq_api.h"
 #include "seq_common.h"
 
@@ -321,7 +323,8 @@ __device__ __forceinline__ uint64_t wide_key(uint32_t key) {
 
 // ---- rows of up to G * N vectors: G lanes a row, all of it in registers
 // Few lanes with up to four vectors each share a row's bookkeeping among few:
-// 524288 x 17 fp32 takes 17 us with 2 lanes of 3 vectors, 25 with 8 of one.
+// 524288 x 17 fp32 takes two thirds of the time with 2 lanes of 3 vectors (16
+// us) that it takes with 8 of one.
 
 // So many lanes or more find a row's alternatives by a bound: 64199 x 886 bf16
 // with 14 takes 57 us so, in rounds 164. Fewer take a round an alternative:
