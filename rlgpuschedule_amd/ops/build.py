@@ -23,6 +23,13 @@ ARCH = os.environ.get("RLS_OFFLOAD_ARCH", "gfx950")
 FLAGS = ["-O3", "-std=c++17", "-fPIC", "-shared",
          "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
+# of the torch bindings, beside the paths of torch and ROCm
+BIND_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-shared",
+              "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+              "-Wl,-rpath,$ORIGIN", "-Wl,--no-as-needed"]
+BIND_LIBS = ["-ltorch", "-ltorch_cpu", "-ltorch_hip", "-lc10", "-lc10_hip",
+             "-ltorch_python"]
+
 # name -> sources
 _LIBS = {
     "librlsched_env.so": ["env_step.hip"],
@@ -50,18 +57,13 @@ def _bind_flags(name: str) -> list[str]:
     root = Path(torch.__file__).resolve().parent
     rocm = Path(HIPCC).resolve().parent.parent
     abi = int(torch.compiled_with_cxx11_abi())
-    return (["-O2", "-std=c++17", "-fPIC", "-shared",
-             "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
-             f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
+    return ([*BIND_FLAGS, f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
              f"-I{sysconfig.get_paths()['include']}"]
             + [f"-isystem{d}" for d in
                (root / "include", root / "include/torch/csrc/api/include",
                 rocm / "include")]
-            + [f"-L{root / 'lib'}", f"-L{OUT}", "-Wl,-rpath,$ORIGIN",
-               "-Wl,--no-as-needed"]
-            + [f"-l:{lib}" for lib in _BINDS[name]]
-            + ["-ltorch", "-ltorch_cpu", "-ltorch_hip", "-lc10", "-lc10_hip",
-               "-ltorch_python"])
+            + [f"-L{root / 'lib'}", f"-L{OUT}"]
+            + [f"-l:{lib}" for lib in _BINDS[name]] + BIND_LIBS)
 
 
 def source_hash(name: str) -> str:
@@ -74,6 +76,7 @@ def source_hash(name: str) -> str:
     if name in _BINDS:
         import torch
         h.update(torch.__version__.encode())
+        h.update(" ".join(BIND_FLAGS + _BINDS[name] + BIND_LIBS).encode())
     srcs = [CSRC / s for s in _LIBS[name]] + sorted(CSRC.glob("*.h"))
     for p in sorted(srcs):
         h.update(p.name.encode())

@@ -319,3 +319,14 @@ def test_threads_that_load_the_bindings_at_once(monkeypatch):
         t.join()
     assert len(got) == 4 and all(m is got[0] for m in got)
     assert sorted(built) == sorted(set(built))
+
+
+def test_bindings_are_built_again_for_other_flags(monkeypatch):
+    from rlgpuschedule_amd.ops import build as B
+    name = "librlsched_seq.so"
+    before = B.source_hash(name)
+    for which in ("BIND_FLAGS", "BIND_LIBS"):
+        with monkeypatch.context() as m:
+            m.setattr(B, which, getattr(B, which) + ["-lm"])
+            assert B.source_hash(name) != before, which
+    assert B.source_hash(name) == before
