@@ -87,8 +87,7 @@ def _packed(t):
 def _may_share(a, b):
     """Whether b may share memory with a, which is contiguous: of views of
     one storage only packed ones apart from it are known not to."""
-    if (not a.numel() or not b.numel() or a.untyped_storage().data_ptr()
-            != b.untyped_storage().data_ptr()):
+    if not (a.numel() and b.numel() and torch._C._is_alias_of(a, b)):
         return False
     if not _packed(b):
         return True

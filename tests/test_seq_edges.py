@@ -330,3 +330,19 @@ def test_bindings_are_built_again_for_other_flags(monkeypatch):
             m.setattr(B, which, getattr(B, which) + ["-lm"])
             assert B.source_hash(name) != before, which
     assert B.source_hash(name) == before
+
+
+def test_shapes_without_data():
+    """Meta and fake tensors, whose storages have no addresses, are not taken
+    for ones that share memory; views of one of them are."""
+    from torch._subclasses import FakeTensorMode
+
+    def steps(gate, x, h):
+        assert gated_scan_step(gate, x, h).shape == (2, 6)
+        assert gated_scan(gate[None], x[None], h)[0].shape == (1, 2, 6)
+        with pytest.raises(ValueError, match="share"):
+            gated_scan_step(h, x, h)
+
+    steps(*(torch.zeros(2, 6, device="meta") for _ in range(3)))
+    with FakeTensorMode():
+        steps(*(torch.zeros(2, 6) for _ in range(3)))
