@@ -71,8 +71,21 @@ void same_device(const Tensor& x, const MaybeTensor& t, const char* name) {
   if (t) same_device(x, *t, name);
 }
 
+// A kernel's view of a tensor's memory. Fake and wrapped tensors, and ones
+// whose storage was freed, have none: torch hands out a null pointer then, or
+// a view's offset from it.
+template <typename P>
+P* backed(P* p, const Tensor& t, const char* name = "a tensor") {
+  if (t.numel() > 0 && !t.storage().data())
+    fail<std::runtime_error>(name, " of shape ", t.sizes(),
+                             " has no memory on the GPU (it is fake, wrapped "
+                             "or freed, or a fake mode is active)");
+  return p;
+}
+
 void on_gpu(const Tensor& x, const char* name) {
   VALUE_CHECK(x.is_cuda(), name, " must be on a GPU, got ", x.device());
+  (void)backed(x.const_data_ptr(), x, name);
 }
 
 struct Place {
@@ -83,11 +96,12 @@ struct Place {
         stream(c10::hip::getCurrentHIPStream(x.get_device()).stream()) {}
 };
 
+const void* ptr(const Tensor& t) { return backed(t.const_data_ptr(), t); }
 const void* ptr(const MaybeTensor& t) {
-  return t && t->defined() ? t->const_data_ptr() : nullptr;
+  return t && t->defined() ? ptr(*t) : nullptr;
 }
 void* out_ptr(const Tensor& t) {
-  return t.defined() ? t.mutable_data_ptr() : nullptr;
+  return t.defined() ? backed(t.mutable_data_ptr(), t) : nullptr;
 }
 float* f32_ptr(const Tensor& t) { return (float*)out_ptr(t); }
 MaybeTensor maybe(const Tensor& t) {
@@ -239,9 +253,9 @@ std::tuple<Tensor, Tensor, Tensor> norm_fwd(const Tensor& x,
   const auto [xr, stride] = rows_of(x);
   const MaybeTensor w = packed(weight), b = packed(bias);
   const Place at(x);
-  done_with(rlsched_norm_fwd(at.device, at.stream, xr.const_data_ptr(), ptr(w),
-                             ptr(b), out_ptr(y), f32_ptr(mean), f32_ptr(rstd),
-                             rows, d, stride, eps, t.x, t.w),
+  done_with(rlsched_norm_fwd(at.device, at.stream, ptr(xr), ptr(w), ptr(b),
+                             out_ptr(y), f32_ptr(mean), f32_ptr(rstd), rows, d,
+                             stride, eps, t.x, t.w),
             "rlsched_norm_fwd");
   return {y, mean, rstd};
 }
@@ -285,12 +299,10 @@ std::tuple<Tensor, Tensor, Tensor> norm_bwd(
   const MaybeTensor w = packed(weight);
   const Place at(x);
   done_with(
-      rlsched_norm_bwd(at.device, at.stream, dyr.const_data_ptr(),
-                       xr.const_data_ptr(), ptr(w),
-                       mean.const_data_ptr<float>(),
-                       rstd.const_data_ptr<float>(), out_ptr(dx), out_ptr(dw),
-                       out_ptr(db), f32_ptr(partial), rows, d, xs, dys, t.x,
-                       t.w),
+      rlsched_norm_bwd(at.device, at.stream, ptr(dyr), ptr(xr), ptr(w),
+                       (const float*)ptr(mean), (const float*)ptr(rstd),
+                       out_ptr(dx), out_ptr(dw), out_ptr(db), f32_ptr(partial),
+                       rows, d, xs, dys, t.x, t.w),
       "rlsched_norm_bwd");
   return {dx, dw, db};
 }
@@ -386,12 +398,11 @@ std::tuple<Tensor, Tensor, Tensor> scan_fwd(const Tensor& gate_,
   const MaybeTensor h0 = packed(h0_), done = packed(done_);
   const Place at(x);
   done_with(
-      rlsched_scan_fwd(at.device, at.stream, gate.const_data_ptr(),
-                       x.const_data_ptr(), (const float*)ptr(h0),
-                       (const uint8_t*)ptr(done), out_ptr(hs),
-                       f32_ptr(h_last), f32_ptr(states), f32_ptr(scratch), T,
-                       E, H, gate.stride(0), gate.stride(1), x.stride(0),
-                       x.stride(1), type),
+      rlsched_scan_fwd(at.device, at.stream, ptr(gate), ptr(x),
+                       (const float*)ptr(h0), (const uint8_t*)ptr(done),
+                       out_ptr(hs), f32_ptr(h_last), f32_ptr(states),
+                       f32_ptr(scratch), T, E, H, gate.stride(0),
+                       gate.stride(1), x.stride(0), x.stride(1), type),
       "rlsched_scan_fwd");
   return {hs, h_last, states};
 }
@@ -429,8 +440,8 @@ std::tuple<Tensor, Tensor, Tensor> scan_bwd(
   const Place at(x);
   done_with(
       rlsched_scan_bwd(at.device, at.stream, ptr(dhs),
-                       (const float*)ptr(dh_last), gate.const_data_ptr(),
-                       x.const_data_ptr(), states.const_data_ptr<float>(),
+                       (const float*)ptr(dh_last), ptr(gate),
+                       ptr(x), (const float*)ptr(states),
                        (const uint8_t*)ptr(done), out_ptr(dgate), out_ptr(dx),
                        f32_ptr(dh0), f32_ptr(scratch), T, E, H,
                        gate.stride(0), gate.stride(1), x.stride(0),
@@ -501,10 +512,10 @@ Tensor scan_step(const Tensor& gate_, const Tensor& x_, Tensor h,
   const Tensor gate = reachable(gate_), x = reachable(x_);
   const MaybeTensor done = packed(done_);
   const Place at(x);
-  done_with(rlsched_scan_step(at.device, at.stream, gate.const_data_ptr(),
-                              x.const_data_ptr(), (const uint8_t*)ptr(done),
-                              f32_ptr(h), out_ptr(hs), E, H, gate.stride(0),
-                              x.stride(0), type),
+  done_with(rlsched_scan_step(at.device, at.stream, ptr(gate), ptr(x),
+                              (const uint8_t*)ptr(done), f32_ptr(h),
+                              out_ptr(hs), E, H, gate.stride(0), x.stride(0),
+                              type),
             "rlsched_scan_step");
   return hs;
 }
@@ -561,9 +572,9 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> logp_fwd(
   const Tensor actions = actions_.contiguous();
   const Place at(logits);
   done_with(
-      rlsched_logp_fwd(at.device, at.stream, xr.const_data_ptr(),
-                       actions.const_data_ptr<int64_t>(),
-                       mask ? (const uint8_t*)mr.const_data_ptr() : nullptr,
+      rlsched_logp_fwd(at.device, at.stream, ptr(xr),
+                       (const int64_t*)ptr(actions),
+                       mask ? (const uint8_t*)ptr(mr) : nullptr,
                        f32_ptr(logp), f32_ptr(entropy), f32_ptr(stats),
                        f32_ptr(top_logp), (int64_t*)out_ptr(top_index),
                        out_ptr(scratch), rows, A, xs, ms, (int)top_k, type),
@@ -604,10 +615,10 @@ Tensor logp_bwd(const MaybeTensor& dlogp_, const MaybeTensor& dentropy_,
   const Place at(logits);
   done_with(
       rlsched_logp_bwd(at.device, at.stream, (const float*)ptr(dlogp),
-                       (const float*)ptr(dentropy), xr.const_data_ptr(),
-                       actions.const_data_ptr<int64_t>(),
-                       mask ? (const uint8_t*)mr.const_data_ptr() : nullptr,
-                       stats.const_data_ptr<float>(), out_ptr(dlogits), rows,
+                       (const float*)ptr(dentropy), ptr(xr),
+                       (const int64_t*)ptr(actions),
+                       mask ? (const uint8_t*)ptr(mr) : nullptr,
+                       (const float*)ptr(stats), out_ptr(dlogits), rows,
                        A, xs, ms, type),
       "rlsched_logp_bwd");
   return dlogits;

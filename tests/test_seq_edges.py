@@ -7,7 +7,11 @@ import torch
 
 from rlgpuschedule_amd import (action_logprobs, gated_scan, gated_scan_step,
                                layer_norm)
+from rlgpuschedule_amd.ops._seq import ext
+from rlgpuschedule_amd.ops.logprob import (action_logprobs_bwd,
+                                           action_logprobs_fwd)
 from rlgpuschedule_amd.ops.norm import layer_norm_bwd, layer_norm_fwd
+from rlgpuschedule_amd.ops.scan import gated_scan_bwd, gated_scan_fwd
 
 from test_seq_ops import (DEVICES, U, close, gen, randn, run_scan,
                           scan_64)
@@ -346,3 +350,78 @@ def test_shapes_without_data():
     steps(*(torch.zeros(2, 6, device="meta") for _ in range(3)))
     with FakeTensorMode():
         steps(*(torch.zeros(2, 6) for _ in range(3)))
+
+
+# --------------------------------------------------- tensors without memory
+def memoryless_calls(x, s, act):
+    """Every entry point on x [4, 6], s [4, 2, 6], act [4]."""
+    f = torch.zeros(4, device=act.device)
+    st = torch.zeros(1, 2, 6, device=act.device)
+    stats = torch.zeros(4, 3, device=act.device)
+    one, two, h = s[0], s[1], st[0]
+    return [
+        lambda: ext().layer_norm(x, None, None, 1e-5),
+        lambda: layer_norm_fwd(x),
+        lambda: layer_norm_bwd(x, x, None, f, f),
+        lambda: ext().gated_scan(s, s, None, None),
+        lambda: gated_scan_fwd(s, s),
+        lambda: gated_scan_bwd(s, None, s, s, st),
+        lambda: ext().gated_scan_step(one, two, h, None),
+        lambda: ext().action_logprobs(x, act, None, 0),
+        lambda: action_logprobs_fwd(x, act, None, 2),
+        lambda: action_logprobs_bwd(f, f, x, act, None, stats),
+    ]
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_fake_tensors_are_refused(grad):
+    """torch hands out null pointers for fake GPU tensors; none is launched
+    on. (Fake tensors need no GPU.)"""
+    from torch._subclasses import FakeTensorMode
+    with FakeTensorMode():
+        x = torch.empty(4, 6, device="cuda", requires_grad=grad)
+        s = torch.empty(4, 2, 6, device="cuda")
+        act = torch.empty(4, dtype=torch.int64, device="cuda")
+        for call in memoryless_calls(x, s, act):
+            with pytest.raises(RuntimeError, match="no memory"):
+                call()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which", ["mode", "freed", "wrapped"])
+def test_tensors_without_memory_are_refused(which):
+    """Real inputs whose outputs would be fake, freed storages, and wrapper
+    subclasses, on the GPU."""
+    import contextlib
+
+    from torch._subclasses import FakeTensorMode
+
+    class Wrapped(torch.Tensor):
+        @staticmethod
+        def __new__(cls, t):
+            return torch.Tensor._make_wrapper_subclass(
+                cls, t.shape, dtype=t.dtype, device=t.device)
+
+        def __init__(self, t):
+            self.t = t
+
+        @classmethod
+        def __torch_dispatch__(cls, f, types, args=(), kwargs=None):
+            args = [a.t if isinstance(a, Wrapped) else a for a in args]
+            return Wrapped(f(*args, **(kwargs or {})))
+
+    x, s = (torch.randn(*n, device="cuda") for n in ((4, 6), (4, 2, 6)))
+    act = torch.zeros(4, dtype=torch.int64, device="cuda")
+    if which == "wrapped":
+        x, s = Wrapped(x), Wrapped(s)
+    calls = memoryless_calls(x, s, act)
+    if which == "freed":
+        x.untyped_storage().resize_(0)
+        s.untyped_storage().resize_(0)
+    mode = FakeTensorMode() if which == "mode" else contextlib.nullcontext()
+    with mode:
+        for call in calls:
+            with pytest.raises(RuntimeError, match="no memory"):
+                call()
+    torch.cuda.synchronize()
+    assert layer_norm(torch.ones(2, 3, device="cuda")).abs().max() == 0
