@@ -71,21 +71,33 @@ void same_device(const Tensor& x, const MaybeTensor& t, const char* name) {
   if (t) same_device(x, *t, name);
 }
 
-// A kernel's view of a tensor's memory. Fake and wrapped tensors, and ones
-// whose storage was freed, have none: torch hands out a null pointer then, or
-// a view's offset from it.
-template <typename P>
-P* backed(P* p, const Tensor& t, const char* name = "a tensor") {
-  if (t.numel() > 0 && !t.storage().data())
-    fail<std::runtime_error>(name, " of shape ", t.sizes(),
-                             " has no memory on the GPU (it is fake, wrapped "
-                             "or freed, or a fake mode is active)");
-  return p;
+// Whether a tensor's storage holds anything. Those of fake and wrapped tensors
+// do not, and what is freed or shrunk keeps its views: torch hands out a
+// pointer for each all the same.
+bool has_memory(const Tensor& t) {
+  return t.numel() == 0 || t.storage().data() != nullptr;
+}
+
+// Whether it reaches as far as the tensor's elements.
+bool has_all_memory(const Tensor& t) {
+  if (t.numel() == 0) return true;
+  if (!has_memory(t)) return false;
+  const auto sizes = t.sizes(), strides = t.strides();
+  int64_t last = t.storage_offset();
+  for (size_t i = 0; i < sizes.size(); ++i) last += (sizes[i] - 1) * strides[i];
+  return (last + 1) * (int64_t)t.element_size() <=
+         (int64_t)t.storage().nbytes();
+}
+
+[[noreturn]] void no_memory(const Tensor& t, const char* name) {
+  fail<std::runtime_error>(name, " of shape ", t.sizes(),
+                           " has no memory on the GPU (it is fake, wrapped or "
+                           "freed, or a fake mode is active)");
 }
 
 void on_gpu(const Tensor& x, const char* name) {
   VALUE_CHECK(x.is_cuda(), name, " must be on a GPU, got ", x.device());
-  (void)backed(x.const_data_ptr(), x, name);
+  if (!has_memory(x)) no_memory(x, name);
 }
 
 struct Place {
@@ -96,12 +108,17 @@ struct Place {
         stream(c10::hip::getCurrentHIPStream(x.get_device()).stream()) {}
 };
 
-const void* ptr(const Tensor& t) { return backed(t.const_data_ptr(), t); }
+const void* ptr(const Tensor& t) {
+  if (!has_all_memory(t)) no_memory(t, "an input");
+  return t.const_data_ptr();
+}
 const void* ptr(const MaybeTensor& t) {
   return t && t->defined() ? ptr(*t) : nullptr;
 }
 void* out_ptr(const Tensor& t) {
-  return t.defined() ? backed(t.mutable_data_ptr(), t) : nullptr;
+  if (!t.defined()) return nullptr;
+  if (!has_memory(t)) no_memory(t, "an output");
+  return t.mutable_data_ptr();
 }
 float* f32_ptr(const Tensor& t) { return (float*)out_ptr(t); }
 MaybeTensor maybe(const Tensor& t) {
@@ -506,6 +523,7 @@ Tensor scan_step(const Tensor& gate_, const Tensor& x_, Tensor h,
                 "h is updated in place: it must not share memory with gate, "
                 "x or done");
   on_gpu(x_, "x");
+  if (!has_all_memory(h)) no_memory(h, "h");
   h.unsafeGetTensorImpl()->bump_version();
   const int64_t E = x_.size(0), H = x_.size(1);
   Tensor hs = at::empty({E, H}, x_.options().requires_grad(false));

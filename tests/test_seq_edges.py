@@ -388,10 +388,10 @@ def test_fake_tensors_are_refused(grad):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("which", ["mode", "freed", "wrapped"])
+@pytest.mark.parametrize("which", ["mode", "freed", "shrunk", "wrapped"])
 def test_tensors_without_memory_are_refused(which):
-    """Real inputs whose outputs would be fake, freed storages, and wrapper
-    subclasses, on the GPU."""
+    """Real inputs whose outputs would be fake, freed and shrunk storages, and
+    wrapper subclasses, on the GPU."""
     import contextlib
 
     from torch._subclasses import FakeTensorMode
@@ -415,9 +415,9 @@ def test_tensors_without_memory_are_refused(which):
     if which == "wrapped":
         x, s = Wrapped(x), Wrapped(s)
     calls = memoryless_calls(x, s, act)
-    if which == "freed":
-        x.untyped_storage().resize_(0)
-        s.untyped_storage().resize_(0)
+    if which in ("freed", "shrunk"):
+        for t in (x, s):  # 10 elements, of which no call's inputs are fewer
+            t.untyped_storage().resize_(0 if which == "freed" else 40)
     mode = FakeTensorMode() if which == "mode" else contextlib.nullcontext()
     with mode:
         for call in calls:
