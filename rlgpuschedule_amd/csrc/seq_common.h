@@ -152,7 +152,7 @@ struct OnDevice {
 
 // The launch's own status: an error left by other code stays where it is.
 // 2^32 lanes or more along one axis are refused here: the runtime refuses
-// 2^32 itself, but a launch of 2^32 + 3072 left most of its work undone
+// 2^32 itself, but a launch of a few blocks more left most of its work undone
 // without an error.
 template <typename... P, typename... A>
 inline hipError_t launch(void (*kernel)(P...), dim3 grid, dim3 block,
