@@ -78,21 +78,23 @@ bool has_memory(const Tensor& t) {
   return t.numel() == 0 || t.storage().data() != nullptr;
 }
 
-// Whether it reaches as far as the tensor's elements.
-bool has_all_memory(const Tensor& t) {
-  if (t.numel() == 0) return true;
-  if (!has_memory(t)) return false;
-  const auto sizes = t.sizes(), strides = t.strides();
-  int64_t last = t.storage_offset();
-  for (size_t i = 0; i < sizes.size(); ++i) last += (sizes[i] - 1) * strides[i];
-  return (last + 1) * (int64_t)t.element_size() <=
-         (int64_t)t.storage().nbytes();
-}
-
 [[noreturn]] void no_memory(const Tensor& t, const char* name) {
   fail<std::runtime_error>(name, " of shape ", t.sizes(),
                            " has no memory on the GPU (it is fake, wrapped or "
                            "freed, or a fake mode is active)");
+}
+
+// An input whose storage reaches as far as its elements: asked before anything,
+// a copy of torch's too, reads it.
+const Tensor& held(const Tensor& t) {
+  if (t.numel() == 0) return t;
+  if (!has_memory(t)) no_memory(t, "an input");
+  const auto sizes = t.sizes(), strides = t.strides();
+  int64_t last = t.storage_offset();
+  for (size_t i = 0; i < sizes.size(); ++i) last += (sizes[i] - 1) * strides[i];
+  if ((last + 1) * (int64_t)t.element_size() > (int64_t)t.storage().nbytes())
+    no_memory(t, "an input");
+  return t;
 }
 
 void on_gpu(const Tensor& x, const char* name) {
@@ -109,7 +111,7 @@ struct Place {
 };
 
 const void* ptr(const Tensor& t) {
-  if (!has_all_memory(t)) no_memory(t, "an input");
+  if (!has_memory(t)) no_memory(t, "an input");
   return t.const_data_ptr();
 }
 const void* ptr(const MaybeTensor& t) {
@@ -126,7 +128,9 @@ MaybeTensor maybe(const Tensor& t) {
 }
 // Values as memory holds them: torch notes a conjugate's imaginary part as to
 // be negated.
-Tensor plain(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
+Tensor plain(const Tensor& t) {
+  return held(t).is_neg() ? t.resolve_neg() : t;
+}
 MaybeTensor packed(const MaybeTensor& t) {
   return t && t->defined() ? MaybeTensor(plain(*t).contiguous())
                            : std::nullopt;
@@ -317,7 +321,8 @@ std::tuple<Tensor, Tensor, Tensor> norm_bwd(
   const Place at(x);
   done_with(
       rlsched_norm_bwd(at.device, at.stream, ptr(dyr), ptr(xr), ptr(w),
-                       (const float*)ptr(mean), (const float*)ptr(rstd),
+                       (const float*)ptr(held(mean)),
+                       (const float*)ptr(held(rstd)),
                        out_ptr(dx), out_ptr(dw), out_ptr(db), f32_ptr(partial),
                        rows, d, xs, dys, t.x, t.w),
       "rlsched_norm_bwd");
@@ -458,7 +463,7 @@ std::tuple<Tensor, Tensor, Tensor> scan_bwd(
   done_with(
       rlsched_scan_bwd(at.device, at.stream, ptr(dhs),
                        (const float*)ptr(dh_last), ptr(gate),
-                       ptr(x), (const float*)ptr(states),
+                       ptr(x), (const float*)ptr(held(states)),
                        (const uint8_t*)ptr(done), out_ptr(dgate), out_ptr(dx),
                        f32_ptr(dh0), f32_ptr(scratch), T, E, H,
                        gate.stride(0), gate.stride(1), x.stride(0),
@@ -523,7 +528,7 @@ Tensor scan_step(const Tensor& gate_, const Tensor& x_, Tensor h,
                 "h is updated in place: it must not share memory with gate, "
                 "x or done");
   on_gpu(x_, "x");
-  if (!has_all_memory(h)) no_memory(h, "h");
+  held(h);
   h.unsafeGetTensorImpl()->bump_version();
   const int64_t E = x_.size(0), H = x_.size(1);
   Tensor hs = at::empty({E, H}, x_.options().requires_grad(false));
@@ -587,7 +592,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> logp_fwd(
   Tensor mr;
   int64_t ms = 0;
   if (mask) std::tie(mr, ms) = rows_of(*mask);
-  const Tensor actions = actions_.contiguous();
+  const Tensor actions = held(actions_).contiguous();
   const Place at(logits);
   done_with(
       rlsched_logp_fwd(at.device, at.stream, ptr(xr),
@@ -629,14 +634,14 @@ Tensor logp_bwd(const MaybeTensor& dlogp_, const MaybeTensor& dentropy_,
   int64_t ms = 0;
   if (mask) std::tie(mr, ms) = rows_of(*mask);
   const MaybeTensor dlogp = packed(dlogp_), dentropy = packed(dentropy_);
-  const Tensor actions = actions_.contiguous();
+  const Tensor actions = held(actions_).contiguous();
   const Place at(logits);
   done_with(
       rlsched_logp_bwd(at.device, at.stream, (const float*)ptr(dlogp),
                        (const float*)ptr(dentropy), ptr(xr),
                        (const int64_t*)ptr(actions),
                        mask ? (const uint8_t*)ptr(mr) : nullptr,
-                       (const float*)ptr(stats), out_ptr(dlogits), rows,
+                       (const float*)ptr(held(stats)), out_ptr(dlogits), rows,
                        A, xs, ms, type),
       "rlsched_logp_bwd");
   return dlogits;

@@ -425,3 +425,39 @@ def test_tensors_without_memory_are_refused(which):
                 call()
     torch.cuda.synchronize()
     assert layer_norm(torch.ones(2, 3, device="cuda")).abs().max() == 0
+
+
+@pytest.mark.gpu
+def test_every_input_is_held():
+    """An input that would be copied first, of each argument in turn, with the
+    end of its storage or all of it gone: refused before the copy."""
+    def t(*size, dtype=torch.float32):
+        return torch.zeros(*size, dtype=dtype, device="cuda")
+
+    calls = [
+        (layer_norm_fwd, [t(4, 6), t(6), t(6)]),
+        (layer_norm_bwd, [t(4, 6), t(4, 6), t(6), t(4), t(4)]),
+        (gated_scan_fwd, [t(4, 2, 6), t(4, 2, 6), t(2, 6),
+                          t(4, 2, dtype=torch.bool)]),
+        (gated_scan_bwd, [t(4, 2, 6), t(2, 6), t(4, 2, 6), t(4, 2, 6),
+                          t(1, 2, 6), t(4, 2, dtype=torch.bool)]),
+        (gated_scan_step, [t(2, 6), t(2, 6), t(2, 6),
+                           t(2, dtype=torch.bool)]),
+        (action_logprobs_fwd, [t(4, 6), t(4, dtype=torch.int64),
+                               t(4, 6, dtype=torch.bool)]),
+        (action_logprobs_bwd, [t(4), t(4), t(4, 6), t(4, dtype=torch.int64),
+                               t(4, 6, dtype=torch.bool), t(4, 3)]),
+    ]
+    whole = {(layer_norm_bwd, 3), (layer_norm_bwd, 4), (gated_scan_bwd, 4),
+             (gated_scan_step, 2), (action_logprobs_bwd, 5)}  # never copied
+    for call, args in calls:
+        call(*args)
+        for i, a in enumerate(args):
+            bad = a.clone()
+            if (call, i) not in whole:
+                bad = torch.stack([bad, bad], -1)[..., 0]  # strides of 2
+            last = sum((n - 1) * s for n, s in zip(bad.shape, bad.stride()))
+            for size in (last * bad.element_size(), 0):  # one short, nothing
+                bad.untyped_storage().resize_(size)
+                with pytest.raises(RuntimeError, match="no memory"):
+                    call(*args[:i], bad, *args[i + 1:])
