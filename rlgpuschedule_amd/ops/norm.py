@@ -2,8 +2,8 @@
 
 `layer_norm` is the differentiable call; `layer_norm_fwd` and
 `layer_norm_bwd` are the explicit pair for learners that capture their
-update. On CPU tensors `layer_norm` runs the torch reference
-(ops/seq_ref.py) after the same checks. Launches go to the current stream of x's device and are
+update. On CPU tensors `layer_norm` runs the torch reference (ops/seq_ref.py)
+after the same checks. Launches go to the current stream of x's device and are
 hipGraph-capturable."""
 from __future__ import annotations
 
